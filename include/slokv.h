@@ -49,6 +49,7 @@ extern "C" {
 #define SLOKV_DTYPE_F16       1
 #define SLOKV_DTYPE_F32       2
 #define SLOKV_DTYPE_FP8_E4M3  3
+#define SLOKV_DTYPE_INT4      4  /* 4-bit pool (slokv_kv_append_int4) */
 
 /* Human-readable text for a status code. */
 const char *slokv_status_string(int status);
@@ -390,6 +391,141 @@ int slokv_kv_block_copy(const void *src, int64_t src_plane_stride_bytes,
                         int32_t dst_capacity,
                         int32_t num_pages, int32_t num_planes, int64_t page_bytes,
                         uint32_t *dev_error, void *stream);
+
+/*
+ * 4-bit KV cache.  No counterpart in the reference engine.
+ *
+ * Pool: one side (K or V) is uint8 [num_blocks, num_kv_heads, block_size * 72],
+ * block_size a multiple of 64, head_dim 128; block strides are in bytes, multiples
+ * of 16, at least num_kv_heads * block_size * 72.  A (block, head) run is tiles of
+ * 64 tokens (4608 bytes): 64 rows of 64 code bytes, then 64 rows of (scale, minimum)
+ * of dims 0-63 and of dims 64-127 in bf16.  Dim 2i of a group is the low and 2i + 1
+ * the high half of byte i of its 32 bytes; the row's 32-bit words alternate between
+ * the two groups (stored word 2i + g is word i of group g).
+ *   value = minimum + scale * code, code in 0 .. 15.
+ *
+ * Quantising append (every step in fp32, round to nearest even):
+ *   scale = bf16((max - min) / 15), minimum = bf16(min),
+ *   code = scale > 0 ? clamp(rint((x - minimum) / scale), 0, 15) : 0.
+ * A group with a NaN or infinity, or whose range overflows fp32, gets a NaN scale
+ * (its values read as NaN) and sets SLOKV_DEVERR_NONFINITE.  Nothing but the stored
+ * tokens' own bytes is written, so a reused page needs no reset.  Slot -1 skips; the
+ * other slots of one call are distinct.  key / value: [tokens, heads, 128] with
+ * row and head strides in elements, in_dtype bf16, f16 or f32, any element-aligned
+ * address (16-byte loads where the addresses allow them).
+ */
+int slokv_kv_append_int4(const void *key, int64_t key_row_stride, int64_t key_head_stride,
+                         const void *value, int64_t value_row_stride, int64_t value_head_stride,
+                         void *k_cache, void *v_cache, int64_t k_block_stride,
+                         int64_t v_block_stride, const int32_t *slot_mapping, int32_t num_tokens,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         int32_t num_blocks, int32_t in_dtype, uint32_t *dev_error, void *stream);
+
+/* Values of single rows: out [num_tokens, num_kv_heads, 128] fp32 (16-byte
+ * aligned), the rows at slot_mapping of one side's pool.  Slot -1 gives zeros; a
+ * slot outside the pool too, with SLOKV_DEVERR_SLOT_RANGE. */
+int slokv_int4_decode(const void *cache, int64_t block_stride, const int32_t *slot_mapping,
+                      int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+                      int32_t block_size, int32_t num_blocks, float *out, uint32_t *dev_error,
+                      void *stream);
+
+/* Prefix-cache prefill over a 4-bit pool: the first cu_seqlens_k[r+1] -
+ * cu_seqlens_k[r] tokens of each row are widened to pages of 128 tokens in
+ * dst_k / dst_v ([num_rows * pages_per_row, 128, num_kv_heads, 128], bf16 or f16),
+ * token t of row r in page r * pages_per_row + t / 128, and dst_table ([num_rows,
+ * pages_per_row]) is filled with those page ids, ready for slokv_paged_prefill
+ * (block_size 128).  Values are rounded once to dst_dtype.  Pages that a row reaches
+ * are written whole (zeros past its keys), the others not at all.  A block id
+ * outside the pool reads as zeros and sets SLOKV_DEVERR_BLOCK_RANGE; keys past the
+ * table's reach set SLOKV_DEVERR_CONTEXT_LEN. */
+int slokv_int4_rows_widen(const void *k_cache, const void *v_cache, int64_t k_block_stride,
+                          int64_t v_block_stride, int32_t num_blocks, int32_t block_size,
+                          int32_t num_kv_heads, int32_t head_dim, const int32_t *block_tables,
+                          int64_t block_table_stride, int32_t max_blocks_per_seq,
+                          const int32_t *cu_seqlens_k, int32_t num_rows, int32_t pages_per_row,
+                          void *dst_k, void *dst_v, int32_t *dst_table, int32_t dst_dtype,
+                          uint32_t *dev_error, void *stream);
+
+/* Paged decode over a 4-bit pool: slokv_paged_decode's arguments and result with
+ * the pool as above.  q / out are bf16 or f16 (q_dtype), at most 16 query heads per
+ * KV head, batch at most 8192.  logits / lse: NULL, or both given as for
+ * slokv_paged_decode_logits.  The workspace holds nothing between calls. */
+size_t slokv_paged_decode_int4_workspace_bytes(int32_t device, int32_t num_q_heads,
+                                               int32_t num_kv_heads, int32_t head_dim);
+int slokv_paged_decode_int4(void *out, int64_t out_stride_b, int64_t out_stride_h, const void *q,
+                            int64_t q_stride_b, int64_t q_stride_h, const void *k_cache,
+                            const void *v_cache, int64_t k_block_stride, int64_t v_block_stride,
+                            int32_t num_blocks, int32_t block_size, int32_t num_q_heads,
+                            int32_t num_kv_heads, int32_t head_dim, const int32_t *block_tables,
+                            int64_t block_table_stride, int32_t max_blocks_per_seq,
+                            const int32_t *context_lens, int32_t batch, float softmax_scale,
+                            int32_t q_dtype, float *logits, int64_t logits_stride, float *lse,
+                            void *workspace, size_t workspace_bytes, uint32_t *dev_error,
+                            void *stream);
+
+/*
+ * Eviction by accumulated attention weight.  No counterpart in the reference engine.
+ *
+ * Scored decode is a decode that also stores its scores, followed by
+ * slokv_kv_scores_accumulate on the same stream:
+ *   logits[b, hq, t] = log2(e) * softmax_scale * q . K[t]   (t < min(L_b, logits_stride))
+ *   lse[b, hq] = log2 sum_t 2^logits[b, hq, t]
+ * slokv_paged_decode_logits: slokv_paged_decode (bf16 / f16 pools) plus logits
+ * ([batch, num_q_heads, logits_stride] fp32) and lse ([batch, num_q_heads] fp32).
+ */
+int slokv_paged_decode_logits(void *out, int64_t out_stride_b, int64_t out_stride_h, const void *q,
+                              int64_t q_stride_b, int64_t q_stride_h, const void *k_cache,
+                              const void *v_cache, int64_t k_block_stride, int64_t v_block_stride,
+                              int32_t num_blocks, int32_t block_size, int32_t num_q_heads,
+                              int32_t num_kv_heads, int32_t head_dim, const int32_t *block_tables,
+                              int64_t block_table_stride, int32_t max_blocks_per_seq,
+                              const int32_t *context_lens, int32_t batch, float softmax_scale,
+                              int32_t dtype, float *logits, int64_t logits_stride, float *lse,
+                              void *workspace, size_t workspace_bytes, uint32_t *dev_error,
+                              void *stream);
+
+/* scores[row, h, t] = decay * scores[row, h, t] + sum over the query heads hq of KV
+ * head h of 2^(logits[b, hq, t] - lse[b, hq]), for t < L_b = context_lens[b], with row =
+ * score_rows ? score_rows[b] : b.  decay 0 overwrites.  scores: fp32
+ * [num_score_rows, num_kv_heads, width] with row and head strides in elements.  A row
+ * of -1 is skipped, one outside [0, num_score_rows) too, with
+ * SLOKV_DEVERR_SLOT_RANGE; two sequences of one call must not share a row.  Positions
+ * past min(width, logits_stride, max_context) are left alone, with
+ * SLOKV_DEVERR_CONTEXT_LEN; max_context: the decode's max_blocks_per_seq * block_size. */
+int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int64_t head_stride,
+                               int32_t width, int32_t num_score_rows, const int32_t *score_rows,
+                               const float *logits, int64_t logits_stride, const float *lse,
+                               const int32_t *context_lens, int32_t batch, int32_t num_q_heads,
+                               int32_t num_kv_heads, int64_t max_context, float decay,
+                               uint32_t *dev_error, void *stream);
+
+/* Evict tokens in place.  For each sequence with L_b > keep and each KV head: the last
+ * `recent` tokens stay, and of the others the keep - recent of the highest score (ties:
+ * the lowest position; NaN counts as -inf).  Kept tokens below position keep stay where they
+ * are; those at or past keep move, in order, into the holes below it -- K row, V row
+ * and score -- and the score row is zeroed from keep to L_b.  new_lens[b] = min(L_b,
+ * keep).  index ([batch, num_kv_heads, keep], may be NULL): the position that each
+ * remaining slot's token came from, -1 past new_lens[b].
+ *
+ * cache_dtype: SLOKV_DTYPE_BF16, _F16, _F32 ([num_blocks, block_size, num_kv_heads, 128])
+ * or _INT4; block strides in bytes; pools 16-byte aligned.  1 <= keep, 0 <= recent
+ * <= keep.  The blocks below position keep must belong to one sequence only (copy
+ * shared ones first).  A sequence whose score row is -1 or outside [0, num_score_rows)
+ * or whose context exceeds the table's or the score row's width is left as it is
+ * (new_lens[b] = L_b), the latter two with SLOKV_DEVERR_SLOT_RANGE / _CONTEXT_LEN; a
+ * move whose block id lies outside the pool is dropped with
+ * SLOKV_DEVERR_BLOCK_RANGE.  new_lens must not overlap context_lens. */
+size_t slokv_kv_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t keep,
+                                      int32_t score_width);
+int slokv_kv_evict(void *k_cache, void *v_cache, int64_t k_block_stride_bytes,
+                   int64_t v_block_stride_bytes, int32_t num_blocks, int32_t block_size,
+                   int32_t num_kv_heads, int32_t head_dim, int32_t cache_dtype,
+                   const int32_t *block_tables, int64_t block_table_stride,
+                   int32_t max_blocks_per_seq, const int32_t *context_lens, int32_t batch,
+                   float *scores, int64_t score_row_stride, int64_t score_head_stride,
+                   int32_t score_width, int32_t num_score_rows, const int32_t *score_rows,
+                   int32_t keep, int32_t recent, int32_t *new_lens, int32_t *index,
+                   void *workspace, size_t workspace_bytes, uint32_t *dev_error, void *stream);
 
 /* ---- row-parallel linear + tensor-parallel all-reduce (one kernel) --------
  *

@@ -16,6 +16,9 @@ from .kvcache import (decode_workspace, e4m3_decode, e4m3_encode, flash_attn_var
                       flash_attn_varlen_func_fp8, flash_attn_with_kvcache, flash_attn_with_kvcache_fp8, kv_block_copy,
                       kv_block_gather, kv_block_scatter, qk_norm_rope_append, store_kvcache,
                       store_kvcache_fp8)
+from .kvcache_int4 import (flash_attn_varlen_func_int4, flash_attn_with_kvcache_int4, int4_decode,
+                           int4_pool_shape, store_kvcache_int4)
+from .eviction import flash_attn_with_kvcache_scored, kv_evict
 from .layers.attention import Attention
 from .layers.linear import RowParallelAllReduce, RowParallelLinear, row_parallel_buffer_bytes
 from .pool import KVPool, block_bytes, plan_num_blocks, tp_shard
@@ -29,6 +32,8 @@ __all__ = [
     "flash_attn_with_kvcache", "flash_attn_with_kvcache_fp8", "forward_mixed",
     "forward_mixed_fp8", "get_context", "store_kvcache_fp8",
     "kv_block_copy", "kv_block_gather", "kv_block_scatter", "qk_norm_rope_append",
+    "flash_attn_varlen_func_int4", "flash_attn_with_kvcache_int4", "int4_decode",
+    "int4_pool_shape", "store_kvcache_int4", "flash_attn_with_kvcache_scored", "kv_evict",
     "read_device_errors", "reset_context", "set_context", "store_kvcache",
     "RowParallelAllReduce", "RowParallelLinear", "row_parallel_buffer_bytes",
 ]

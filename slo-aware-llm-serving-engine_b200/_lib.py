@@ -34,6 +34,7 @@ DTYPE_BF16 = 0
 DTYPE_F16 = 1
 DTYPE_F32 = 2
 DTYPE_FP8_E4M3 = 3
+DTYPE_INT4 = 4
 
 _c_i32, _c_i64, _c_f32, _c_sz, _c_vp = (ctypes.c_int32, ctypes.c_int64, ctypes.c_float,
                                          ctypes.c_size_t, ctypes.c_void_p)
@@ -109,6 +110,38 @@ SIGNATURES = {
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp, _c_i64, _c_i32, _c_vp, _c_i32,
         _c_f32, _c_i32, _c_vp, _c_vp]),   # as slokv_paged_decode, without the workspace
     "slokv_paged_decode_noalloc_scratch_bytes": (_c_sz, []),
+    "slokv_kv_append_int4": (ctypes.c_int, [
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64,   # key, value, row / head strides
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_vp,            # caches, block strides, slots
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,  # T, Hkv, D, bs, blocks, dtype
+        _c_vp, _c_vp]),                                 # dev_error, stream
+    "slokv_int4_decode": (ctypes.c_int, [
+        _c_vp, _c_i64, _c_vp, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp, _c_vp, _c_vp]),
+    "slokv_int4_rows_widen": (ctypes.c_int, [
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,   # pool
+        _c_vp, _c_i64, _c_i32, _c_vp, _c_i32, _c_i32,   # tables, stride, width, cu_k, rows, pages
+        _c_vp, _c_vp, _c_vp, _c_i32, _c_vp, _c_vp]),    # dst k / v / table, dtype, err, stream
+    "slokv_paged_decode_int4_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32]),
+    "slokv_paged_decode_int4": (ctypes.c_int, [
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64,
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp, _c_i64, _c_i32, _c_vp, _c_i32,
+        _c_f32, _c_i32, _c_vp, _c_i64, _c_vp,           # scale, dtype, logits, stride, lse
+        _c_vp, _c_sz, _c_vp, _c_vp]),
+    "slokv_paged_decode_logits": (ctypes.c_int, [
+        _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64,
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp, _c_i64, _c_i32, _c_vp, _c_i32,
+        _c_f32, _c_i32, _c_vp, _c_i64, _c_vp, _c_vp, _c_sz, _c_vp, _c_vp]),
+    "slokv_kv_scores_accumulate": (ctypes.c_int, [
+        _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_vp,   # scores, strides, width, rows, map
+        _c_vp, _c_i64, _c_vp, _c_vp, _c_i32, _c_i32, _c_i32,   # logits, lse, lens, B, Hq, Hkv
+        _c_i64, _c_f32, _c_vp, _c_vp]),                 # max context, decay, err, stream
+    "slokv_kv_evict_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32]),
+    "slokv_kv_evict": (ctypes.c_int, [
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,   # pool
+        _c_vp, _c_i64, _c_i32, _c_vp, _c_i32,           # tables, stride, width, lens, batch
+        _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_vp,   # scores, strides, width, rows, map
+        _c_i32, _c_i32, _c_vp, _c_vp,                   # keep, recent, new_lens, index
+        _c_vp, _c_sz, _c_vp, _c_vp]),                   # workspace, bytes, err, stream
     "slokv_row_parallel_buffer_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32]),
     "slokv_row_parallel_plan": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp]),
     "slokv_row_parallel_linear": (ctypes.c_int, [

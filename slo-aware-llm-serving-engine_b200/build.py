@@ -25,18 +25,22 @@ SOURCES = [
     "paged_decode.cu",
     "kv_block_copy.cu",
     "kv_append_fp8.cu",
+    "kv_append_int4.cu",
+    "paged_decode_int4.cu",
+    "kv_scores.cu",
+    "kv_evict.cu",
     "paged_prefill.cu",
     "qk_norm_rope.cu",
     "fp8_pages_dequant.cu",
     "row_parallel.cu",
 ]
-HEADERS = ["common.cuh", "fp8_e4m3.cuh", "tcgen05.cuh"]
+HEADERS = ["common.cuh", "decode_worklist.cuh", "fp8_e4m3.cuh", "int4_page.cuh", "tcgen05.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
-    "-cudart", "static",
+    "-cudart", "static", "--threads", "0",
 ]
 
 

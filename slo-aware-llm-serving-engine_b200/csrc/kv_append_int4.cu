@@ -1,0 +1,337 @@
+// Quantising paged append to the 4-bit KV pool, the read-back of single rows and the
+// widening of cached rows for prefill.
+//
+// Contract, per token, kv head and group of 64 dims (every step IEEE fp32):
+//   mn = min x, mx = max x
+//   scale = bf16((mx - mn) / 15), minimum = bf16(mn)
+//   code = scale > 0 ? clamp(rint((x - minimum) / scale), 0, 15) : 0
+// A group with a NaN or an infinity, or whose range overflows fp32, is stored with a
+// NaN scale (its values read as NaN) and flags SLOKV_DEVERR_NONFINITE.  A token's
+// parameters are its own, so nothing stored before is touched and a page needs no
+// reset when it changes hands.
+//
+// Mapping: half a warp per row of 128 dims, 8 dims a lane: one 16-byte load, a
+// three-step shuffle min / max over the 8 lanes of a group, one 32-bit word of
+// codes stored (the half warp's words are the row's 64 contiguous bytes).  Neighbouring
+// half warps take K and V of one (token, head), then the next head.
+#include "common.cuh"
+#include "int4_page.cuh"
+
+namespace slokv {
+namespace {
+
+using namespace kv4;
+
+constexpr int kThreads = 256;
+constexpr int kRowsPerCta = kThreads / 16;
+
+template <typename T>
+__device__ __forceinline__ float widen(T x);
+template <>
+__device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float widen<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float widen<float>(float x) { return x; }
+
+// Eight consecutive elements of a row; kVec: the address is 16-byte aligned.
+template <typename T, bool kVec>
+__device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
+  if constexpr (kVec && sizeof(T) == 2) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p));
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = widen(e[i]);
+  } else if constexpr (kVec) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+    const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = widen(p[i]);
+  }
+}
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kThreads)
+    kv_append_int4_kernel(const T *__restrict__ key, int64_t key_stride, int64_t key_head,
+                          const T *__restrict__ value, int64_t value_stride, int64_t value_head,
+                          uint8_t *__restrict__ k_cache, uint8_t *__restrict__ v_cache,
+                          int64_t k_block_stride, int64_t v_block_stride,
+                          const int32_t *__restrict__ slots, int32_t tokens, int32_t hkv,
+                          int32_t block_size, int32_t num_blocks, uint32_t *err) {
+  const int lane = threadIdx.x & 31, sub = lane & 15;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 4);
+  const int64_t rows = static_cast<int64_t>(tokens) * hkv * 2;
+  // every lane takes part in the shuffles; `live` guards the memory accesses
+  bool live = row < rows;
+  const bool is_v = row & 1;
+  const int64_t th = row >> 1;
+  const int32_t t = live ? static_cast<int32_t>(th / hkv) : 0;
+  const int32_t h = live ? static_cast<int32_t>(th - static_cast<int64_t>(t) * hkv) : 0;
+  const int32_t slot = live ? __ldg(slots + t) : -1;
+  if (slot < 0 || slot / block_size >= num_blocks) {
+    if (live && slot != -1 && sub == 0) record_error(err, SLOKV_DEVERR_SLOT_RANGE);
+    live = false;
+  }
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    const T *src = is_v ? value + t * value_stride + h * value_head
+                        : key + t * key_stride + h * key_head;
+    load8<T, kVec>(src + sub * 8, x);
+  }
+  float mn = x[0], mx = x[0];
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    mn = fminf(mn, x[i]);
+    mx = fmaxf(mx, x[i]);
+    bad |= !isfinite(x[i]);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  const uint32_t votes = __ballot_sync(0xffffffffu, bad);
+  bad = (votes >> (lane & 24)) & 0xffu;
+  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(mx, mn), 15.f));
+  const __nv_bfloat16 mb = __float2bfloat16_rn(mn);
+  const float s = __bfloat162float(sb), m = __bfloat162float(mb);
+  bad |= !isfinite(s) || !isfinite(m);
+  uint32_t word = 0;
+  if (!bad && s > 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = rintf(__fdiv_rn(__fsub_rn(x[i], m), s));
+      word |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
+    }
+  }
+  if (!live) return;
+  const int32_t blk = slot / block_size, off = slot - blk * block_size;
+  uint8_t *run = (is_v ? v_cache + blk * v_block_stride : k_cache + blk * k_block_stride) +
+                 static_cast<int64_t>(h) * block_size * kRowBytes;
+  const int grp = sub >> 3, i = sub & 7;
+  *reinterpret_cast<uint32_t *>(run + code_offset(off) + (2 * i + grp) * 4) = word;
+  if (i == 0) {
+    const uint32_t lo = bad ? 0x7fffu : __bfloat16_as_ushort(sb);
+    const uint32_t hi = bad ? 0u : __bfloat16_as_ushort(mb);
+    *reinterpret_cast<uint32_t *>(run + param_offset(off) + 4 * grp) = lo | (hi << 16);
+    if (bad) record_error(err, SLOKV_DEVERR_NONFINITE);
+  }
+}
+
+// The 8 values of natural word (group, i) of a row.
+__device__ __forceinline__ void row_values(const uint8_t *run, int32_t off, int grp, int i,
+                                           float (&v)[8]) {
+  const uint32_t w =
+      __ldg(reinterpret_cast<const uint32_t *>(run + code_offset(off) + (2 * i + grp) * 4));
+  const uint32_t pw = __ldg(reinterpret_cast<const uint32_t *>(run + param_offset(off) + 4 * grp));
+  const float s = scale_of(pw), m = min_of(pw);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = fmaf(s, static_cast<float>((w >> (4 * k)) & 15u), m);
+}
+
+// fp32 values of the rows at `slots` (-1 or outside the pool: zeros), half a warp a row.
+__global__ void __launch_bounds__(kThreads)
+    int4_decode_kernel(const uint8_t *__restrict__ cache, int64_t block_stride,
+                       const int32_t *__restrict__ slots, int32_t tokens, int32_t hkv,
+                       int32_t block_size, int32_t num_blocks, float *__restrict__ out,
+                       uint32_t *err) {
+  const int sub = threadIdx.x & 15;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 4);
+  if (row >= static_cast<int64_t>(tokens) * hkv) return;
+  const int32_t t = static_cast<int32_t>(row / hkv), h = static_cast<int32_t>(row % hkv);
+  const int32_t slot = __ldg(slots + t);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (slot >= 0 && slot / block_size < num_blocks) {
+    const int32_t blk = slot / block_size;
+    row_values(cache + blk * block_stride + static_cast<int64_t>(h) * block_size * kRowBytes,
+               slot - blk * block_size, sub >> 3, sub & 7, v);
+  } else if (slot != -1 && sub == 0) {
+    record_error(err, SLOKV_DEVERR_SLOT_RANGE);
+  }
+  float4 *o = reinterpret_cast<float4 *>(out + row * kHeadDim + sub * 8);
+  o[0] = make_float4(v[0], v[1], v[2], v[3]);
+  o[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Widen the cached tokens of a prefill call's rows to bf16 / f16: token t of row r goes to
+// page r * pages + t / 128 of 128-token pages [.., 128, hkv, 128], whose table is written
+// beside them.  One CTA per (page, head, side).  A page that the row reaches is
+// written whole (zeros past its last key and for a block id outside the pool: the
+// prefill loads whole pages); the others are left alone.
+constexpr int kWidePage = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    int4_rows_widen_kernel(const uint8_t *__restrict__ k_cache, const uint8_t *__restrict__ v_cache,
+                           int64_t k_block_stride, int64_t v_block_stride, int32_t num_blocks,
+                           int32_t block_size, int32_t hkv, const int32_t *__restrict__ tables,
+                           int64_t bt_stride, int32_t max_blocks, const int32_t *__restrict__ cu_k,
+                           int32_t pages, T *__restrict__ dst_k, T *__restrict__ dst_v,
+                           int32_t *__restrict__ dst_table, uint32_t *err) {
+  const int32_t page = blockIdx.x % pages, r = blockIdx.x / pages;
+  const int32_t h = blockIdx.y;
+  const bool is_v = blockIdx.z;
+  const bool first = h == 0 && !is_v && threadIdx.x == 0;
+  if (first) dst_table[blockIdx.x] = blockIdx.x;
+  int64_t keys = static_cast<int64_t>(__ldg(cu_k + r + 1)) - __ldg(cu_k + r);
+  const int64_t reach = static_cast<int64_t>(max_blocks) * block_size;
+  if (keys > reach) {
+    if (first && page == 0) record_error(err, SLOKV_DEVERR_CONTEXT_LEN);
+    keys = reach;
+  }
+  const int64_t t0 = static_cast<int64_t>(page) * kWidePage;
+  if (t0 >= keys) return;
+  const uint8_t *cache = is_v ? v_cache : k_cache;
+  const int64_t stride = is_v ? v_block_stride : k_block_stride;
+  T *dst = (is_v ? dst_v : dst_k) +
+           (static_cast<int64_t>(blockIdx.x) * kWidePage * hkv + h) * kHeadDim;
+  const int sub = threadIdx.x & 15;
+#pragma unroll 4
+  for (int32_t i = threadIdx.x >> 4; i < kWidePage; i += kRowsPerCta) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const int64_t t = t0 + i;
+    if (t < keys) {
+      const int32_t col = static_cast<int32_t>(t / block_size);
+      const int32_t blk = __ldg(tables + r * bt_stride + col);
+      if (blk >= 0 && blk < num_blocks)
+        row_values(cache + blk * stride + static_cast<int64_t>(h) * block_size * kRowBytes,
+                   static_cast<int32_t>(t - static_cast<int64_t>(col) * block_size), sub >> 3,
+                   sub & 7, v);
+      else if (sub == 0)
+        record_error(err, SLOKV_DEVERR_BLOCK_RANGE);
+    }
+    uint4 w;
+    w.x = Mma<T>::pack(v[0], v[1]);
+    w.y = Mma<T>::pack(v[2], v[3]);
+    w.z = Mma<T>::pack(v[4], v[5]);
+    w.w = Mma<T>::pack(v[6], v[7]);
+    *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(i) * hkv * kHeadDim + sub * 8) = w;
+  }
+}
+
+bool pool_ok(const void *base, int64_t block_stride, int32_t hkv, int32_t block_size) {
+  return !(reinterpret_cast<uintptr_t>(base) & 15u) && !(block_stride & 15) &&
+         block_stride >= static_cast<int64_t>(hkv) * block_size * kRowBytes;
+}
+
+// Whether every row's 8-element pieces lie on 16-byte boundaries.
+bool vec_ok(const void *p, int64_t stride, int64_t head, int elem) {
+  return !(reinterpret_cast<uintptr_t>(p) & 15u) && !((stride * elem) & 15) && !((head * elem) & 15);
+}
+
+}  // namespace
+}  // namespace slokv
+
+extern "C" int slokv_kv_append_int4(const void *key, int64_t key_row_stride,
+                                    int64_t key_head_stride, const void *value,
+                                    int64_t value_row_stride, int64_t value_head_stride,
+                                    void *k_cache, void *v_cache, int64_t k_block_stride,
+                                    int64_t v_block_stride, const int32_t *slot_mapping,
+                                    int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t block_size, int32_t num_blocks, int32_t in_dtype,
+                                    uint32_t *dev_error, void *stream) {
+  using namespace slokv;
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_blocks <= 0 || block_size <= 0)
+    return SLOKV_ERR_INVALID_ARG;
+  if (head_dim != kHeadDim || block_size % kTileTokens) return SLOKV_ERR_UNSUPPORTED;
+  if (in_dtype != SLOKV_DTYPE_BF16 && in_dtype != SLOKV_DTYPE_F16 && in_dtype != SLOKV_DTYPE_F32)
+    return SLOKV_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return SLOKV_OK;
+  if (!key || !value || !k_cache || !v_cache || !slot_mapping) return SLOKV_ERR_INVALID_ARG;
+  if (!pool_ok(k_cache, k_block_stride, num_kv_heads, block_size) ||
+      !pool_ok(v_cache, v_block_stride, num_kv_heads, block_size))
+    return SLOKV_ERR_ALIGNMENT;
+  const int elem = in_dtype == SLOKV_DTYPE_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & (elem - 1))
+    return SLOKV_ERR_ALIGNMENT;
+  const int64_t rows = static_cast<int64_t>(num_tokens) * num_kv_heads * 2;
+  const int64_t ctas = (rows + kRowsPerCta - 1) / kRowsPerCta;
+  if (ctas > 0x7fffffff) return SLOKV_ERR_UNSUPPORTED;
+  const bool vec = vec_ok(key, key_row_stride, key_head_stride, elem) &&
+                   vec_ok(value, value_row_stride, value_head_stride, elem);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel, auto tag) {
+    using T = decltype(tag);
+    kernel<<<static_cast<unsigned>(ctas), kThreads, 0, st>>>(
+        static_cast<const T *>(key), key_row_stride, key_head_stride,
+        static_cast<const T *>(value), value_row_stride, value_head_stride,
+        static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_block_stride,
+        v_block_stride, slot_mapping, num_tokens, num_kv_heads, block_size, num_blocks, dev_error);
+    return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
+  };
+  if (in_dtype == SLOKV_DTYPE_BF16)
+    return vec ? go(kv_append_int4_kernel<__nv_bfloat16, true>, __nv_bfloat16())
+               : go(kv_append_int4_kernel<__nv_bfloat16, false>, __nv_bfloat16());
+  if (in_dtype == SLOKV_DTYPE_F16)
+    return vec ? go(kv_append_int4_kernel<__half, true>, __half())
+               : go(kv_append_int4_kernel<__half, false>, __half());
+  return vec ? go(kv_append_int4_kernel<float, true>, float())
+             : go(kv_append_int4_kernel<float, false>, float());
+}
+
+extern "C" int slokv_int4_decode(const void *cache, int64_t block_stride,
+                                 const int32_t *slot_mapping, int32_t num_tokens,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                 int32_t num_blocks, float *out, uint32_t *dev_error,
+                                 void *stream) {
+  using namespace slokv;
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_blocks <= 0 || block_size <= 0)
+    return SLOKV_ERR_INVALID_ARG;
+  if (head_dim != kHeadDim || block_size % kTileTokens) return SLOKV_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return SLOKV_OK;
+  if (!cache || !slot_mapping || !out) return SLOKV_ERR_INVALID_ARG;
+  if (!pool_ok(cache, block_stride, num_kv_heads, block_size) ||
+      (reinterpret_cast<uintptr_t>(out) & 15u))
+    return SLOKV_ERR_ALIGNMENT;
+  const int64_t rows = static_cast<int64_t>(num_tokens) * num_kv_heads;
+  const int64_t ctas = (rows + kRowsPerCta - 1) / kRowsPerCta;
+  if (ctas > 0x7fffffff) return SLOKV_ERR_UNSUPPORTED;
+  int4_decode_kernel<<<static_cast<unsigned>(ctas), kThreads, 0,
+                       static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t *>(cache), block_stride, slot_mapping, num_tokens, num_kv_heads,
+      block_size, num_blocks, out, dev_error);
+  return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
+}
+
+extern "C" int slokv_int4_rows_widen(const void *k_cache, const void *v_cache,
+                                     int64_t k_block_stride, int64_t v_block_stride,
+                                     int32_t num_blocks, int32_t block_size, int32_t num_kv_heads,
+                                     int32_t head_dim, const int32_t *block_tables,
+                                     int64_t block_table_stride, int32_t max_blocks_per_seq,
+                                     const int32_t *cu_seqlens_k, int32_t num_rows,
+                                     int32_t pages_per_row, void *dst_k, void *dst_v,
+                                     int32_t *dst_table, int32_t dst_dtype, uint32_t *dev_error,
+                                     void *stream) {
+  using namespace slokv;
+  if (num_rows < 0 || pages_per_row < 0 || num_kv_heads <= 0 || num_blocks <= 0 || block_size <= 0)
+    return SLOKV_ERR_INVALID_ARG;
+  if (head_dim != kHeadDim || block_size % kTileTokens) return SLOKV_ERR_UNSUPPORTED;
+  if (dst_dtype != SLOKV_DTYPE_BF16 && dst_dtype != SLOKV_DTYPE_F16) return SLOKV_ERR_UNSUPPORTED;
+  if (num_rows == 0 || pages_per_row == 0) return SLOKV_OK;
+  if (!k_cache || !v_cache || !block_tables || !cu_seqlens_k || !dst_k || !dst_v || !dst_table ||
+      max_blocks_per_seq <= 0)
+    return SLOKV_ERR_INVALID_ARG;
+  if (!pool_ok(k_cache, k_block_stride, num_kv_heads, block_size) ||
+      !pool_ok(v_cache, v_block_stride, num_kv_heads, block_size) ||
+      ((reinterpret_cast<uintptr_t>(dst_k) | reinterpret_cast<uintptr_t>(dst_v)) & 15u))
+    return SLOKV_ERR_ALIGNMENT;
+  const int64_t pages = static_cast<int64_t>(num_rows) * pages_per_row;
+  if (pages > 0x7fffffff || num_kv_heads > 65535) return SLOKV_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(pages), static_cast<unsigned>(num_kv_heads), 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel, auto tag) {
+    using T = decltype(tag);
+    kernel<<<grid, kThreads, 0, st>>>(
+        static_cast<const uint8_t *>(k_cache), static_cast<const uint8_t *>(v_cache),
+        k_block_stride, v_block_stride, num_blocks, block_size, num_kv_heads, block_tables,
+        block_table_stride, max_blocks_per_seq, cu_seqlens_k, pages_per_row,
+        static_cast<T *>(dst_k), static_cast<T *>(dst_v), dst_table, dev_error);
+    return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
+  };
+  return dst_dtype == SLOKV_DTYPE_BF16 ? go(int4_rows_widen_kernel<__nv_bfloat16>, __nv_bfloat16())
+                                       : go(int4_rows_widen_kernel<__half>, __half());
+}

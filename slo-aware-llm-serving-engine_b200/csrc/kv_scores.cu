@@ -1,0 +1,140 @@
+// Accumulated attention weights of cached keys, the second half of the scored decode:
+//
+//   scores[row, h, t] = decay * scores[row, h, t] + sum_{g in group h} 2^(x[g, t] - lse[g])
+//
+// x and lse are the log2-domain scores and denominators that the decode kernels store
+// (4 G bytes a token and head against the K and V rows' 144 to 512, so that K is not
+// read a second time).  One thread takes four tokens of one head and adds its group
+// in order: no atomics, the same sum on every run.
+#include "common.cuh"
+
+namespace slokv {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPer = 4;  // tokens of a thread
+
+struct ScoreParams {
+  float *scores;
+  int64_t row_stride, head_stride;
+  int32_t width, num_rows;
+  const int32_t *rows;
+  const float *logits;
+  int64_t logits_stride;
+  const float *lse;
+  const int32_t *lens;
+  int32_t hkv, group, cap;
+  float decay;
+  uint32_t *err;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// kVec: score and logit rows allow 16-byte accesses.
+template <bool kVec>
+__global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const ScoreParams p) {
+  const int32_t b = blockIdx.z, h = blockIdx.y;
+  int32_t len = __ldg(p.lens + b);
+  const int32_t row = p.rows ? __ldg(p.rows + b) : b;
+  const bool first = blockIdx.x == 0 && h == 0 && threadIdx.x == 0;
+  if (row < 0 || row >= p.num_rows) {
+    if (first && row != -1) record_error(p.err, SLOKV_DEVERR_SLOT_RANGE);
+    return;
+  }
+  if (len > p.cap) {
+    if (first) record_error(p.err, SLOKV_DEVERR_CONTEXT_LEN);
+    len = p.cap;
+  }
+  const int32_t t = (blockIdx.x * kThreads + threadIdx.x) * kPer;
+  if (t >= len) return;
+  const int32_t n = min(kPer, len - t);
+  const float *lg =
+      p.logits + (static_cast<int64_t>(b) * p.hkv + h) * p.group * p.logits_stride + t;
+  const float *lse = p.lse + (static_cast<int64_t>(b) * p.hkv + h) * p.group;
+  float w[kPer] = {0.f, 0.f, 0.f, 0.f};
+  for (int g = 0; g < p.group; ++g, lg += p.logits_stride) {
+    const float d = __ldg(lse + g);
+    if (d == -INFINITY) continue;  // a head whose every score is -inf has no weights
+    float x[kPer];
+    if (kVec && n == kPer) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(lg));
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = i < n ? __ldg(lg + i) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) w[i] += exp2_fast(x[i] - d);
+  }
+  float *s = p.scores + row * p.row_stride + h * p.head_stride + t;
+  if (kVec && n == kPer) {
+    if (p.decay != 0.f) {
+      const float4 v = *reinterpret_cast<const float4 *>(s);
+      w[0] = fmaf(p.decay, v.x, w[0]);
+      w[1] = fmaf(p.decay, v.y, w[1]);
+      w[2] = fmaf(p.decay, v.z, w[2]);
+      w[3] = fmaf(p.decay, v.w, w[3]);
+    }
+    *reinterpret_cast<float4 *>(s) = make_float4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i < n) s[i] = p.decay != 0.f ? fmaf(p.decay, s[i], w[i]) : w[i];
+  }
+}
+
+}  // namespace
+}  // namespace slokv
+
+extern "C" int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int64_t head_stride,
+                                          int32_t width, int32_t num_score_rows,
+                                          const int32_t *score_rows, const float *logits,
+                                          int64_t logits_stride, const float *lse,
+                                          const int32_t *context_lens, int32_t batch,
+                                          int32_t num_q_heads, int32_t num_kv_heads,
+                                          int64_t max_context, float decay, uint32_t *dev_error,
+                                          void *stream) {
+  using namespace slokv;
+  if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
+      width < 0 || num_score_rows < 0 || max_context < 0)
+    return SLOKV_ERR_INVALID_ARG;
+  if (batch == 0 || width == 0) return SLOKV_OK;
+  if (!scores || !logits || !lse || !context_lens || logits_stride <= 0)
+    return SLOKV_ERR_INVALID_ARG;
+  if (batch > 65535 || num_kv_heads > 65535) return SLOKV_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(logits)) & 3u)
+    return SLOKV_ERR_ALIGNMENT;
+  ScoreParams p;
+  p.scores = scores;
+  p.row_stride = row_stride;
+  p.head_stride = head_stride;
+  p.width = width;
+  p.num_rows = num_score_rows;
+  p.rows = score_rows;
+  p.logits = logits;
+  p.logits_stride = logits_stride;
+  p.lse = lse;
+  p.lens = context_lens;
+  p.hkv = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
+  int64_t cap = width < logits_stride ? width : logits_stride;
+  if (max_context < cap) cap = max_context;
+  p.cap = static_cast<int32_t>(cap);
+  p.decay = decay;
+  p.err = dev_error;
+  if (cap == 0) return SLOKV_OK;
+  const bool vec = !((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(logits)) & 15u) &&
+                   !((row_stride | head_stride | logits_stride) & 3);
+  const dim3 grid(static_cast<unsigned>((cap + kThreads * kPer - 1) / (kThreads * kPer)),
+                  static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (vec)
+    kv_scores_accumulate_kernel<true><<<grid, kThreads, 0, st>>>(p);
+  else
+    kv_scores_accumulate_kernel<false><<<grid, kThreads, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
+}

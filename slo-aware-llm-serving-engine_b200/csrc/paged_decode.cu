@@ -25,6 +25,7 @@
 //    workspace, which a small merge kernel combines.  At most two partials per
 //    warp exist, so the workspace does not depend on batch or context length.
 #include "common.cuh"
+#include "decode_worklist.cuh"
 #include "fp8_e4m3.cuh"
 
 #include <cudaTypedefs.h>
@@ -35,14 +36,10 @@
 namespace slokv {
 namespace decode {
 
-constexpr int kD = 128;                         // head_dim
 constexpr int kTile = 32;                       // tokens per pipeline stage
 constexpr int kHalfBytes = kTile * 128;         // 32 rows x 64 dims x 2 B
 constexpr int kStageBytes = 4 * kHalfBytes;     // K lo/hi + V lo/hi halves
 constexpr int kRingBytes = 192 * 1024;          // K/V stages of all warps of a CTA
-constexpr int kRowFloats = kD + 4;              // partial row: m, l, pad, pad, acc[kD]
-constexpr int kAccOff = 4;                      // acc starts 16-byte aligned
-constexpr int kMaxBatch = 8192;
 
 struct Params {
   void *out;
@@ -62,105 +59,10 @@ struct Params {
   int4 *jobs;       // [nslots]: merge job of the warp slot (x = -1: none)
   uint32_t *err;
   int32_t nslots;
+  float *logits;    // scored decode: [batch, hq, logits_stride] log2-domain scores
+  float *lse;       // scored decode: [batch, hq] log2 of the softmax denominator
+  int64_t logits_stride;
 };
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Number of tiles of sequence b (its segment length per kv head).
-__device__ __forceinline__ int32_t seq_tiles(const Params &p, int b, uint32_t *err_bits) {
-  int32_t len = __ldg(p.context_lens + b);
-  if (len <= 0) return 0;
-  const int32_t cap = p.max_blocks * p.block_size;
-  if (len > cap) {
-    *err_bits |= SLOKV_DEVERR_CONTEXT_LEN;
-    len = cap;
-  }
-  return (len + kTile - 1) / kTile;
-}
-
-__device__ __forceinline__ int32_t seq_len_clamped(const Params &p, int b) {
-  int32_t len = __ldg(p.context_lens + b);
-  const int32_t cap = p.max_blocks * p.block_size;
-  return len > cap ? cap : len;
-}
-
-// Exclusive prefix over sequences of (tiles_b * hkv) into prefix[0..batch].
-// Called by all threads of the CTA.
-__device__ void build_prefix(const Params &p, int32_t *prefix, uint32_t *err_bits) {
-  __shared__ int32_t warp_sums[32];
-  const int tid = threadIdx.x, nthr = blockDim.x;
-  const int per = (p.batch + nthr - 1) / nthr;
-  const int lo = min(tid * per, p.batch), hi = min(lo + per, p.batch);
-  int32_t local = 0;
-  for (int b = lo; b < hi; ++b) local += seq_tiles(p, b, err_bits) * p.hkv;
-  // inclusive scan of `local` across the CTA
-  const int lane = tid & 31, warp = tid >> 5;
-  int32_t v = local;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    int32_t t = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += t;
-  }
-  if (lane == 31) warp_sums[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    const int nw = nthr >> 5;
-    int32_t w = lane < nw ? warp_sums[lane] : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      int32_t t = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += t;
-    }
-    if (lane < nw) warp_sums[lane] = w;
-  }
-  __syncthreads();
-  int32_t run = v - local + (warp > 0 ? warp_sums[warp - 1] : 0);
-  for (int b = lo; b < hi; ++b) {
-    prefix[b] = run;
-    uint32_t dummy = 0;
-    run += seq_tiles(p, b, &dummy) * p.hkv;
-  }
-  if (tid == nthr - 1) prefix[p.batch] = run;
-  __syncthreads();
-}
-
-struct TileRef {
-  int32_t b, h, j, nt, seg_start;
-};
-
-// Locate global tile t: largest b with prefix[b] <= t.
-__device__ __forceinline__ TileRef locate(const Params &p, const int32_t *prefix, int64_t t) {
-  int lo = 0, hi = p.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (prefix[mid] <= t) lo = mid; else hi = mid - 1;
-  }
-  TileRef r;
-  r.b = lo;
-  r.nt = (prefix[lo + 1] - prefix[lo]) / p.hkv;
-  const int32_t rel = static_cast<int32_t>(t - prefix[lo]);
-  r.h = rel / r.nt;
-  r.j = rel - r.h * r.nt;
-  r.seg_start = prefix[lo] + r.h * r.nt;
-  return r;
-}
-
-__device__ __forceinline__ int64_t range_start(int64_t s, int64_t total, int64_t nslots) {
-  return (s * total) / nslots;
-}
-
-// Slot that owns global tile t (max s with range_start(s) <= t).
-__device__ __forceinline__ int64_t owner_slot(int64_t t, int64_t total, int64_t nslots) {
-  int64_t s = (t * nslots) / total;
-  if (s >= nslots) s = nslots - 1;
-  while (s + 1 < nslots && range_start(s + 1, total, nslots) <= t) ++s;
-  while (s > 0 && range_start(s, total, nslots) > t) --s;
-  return s;
-}
 
 // The next tile a warp's producer lane issues, advanced tile by tile in the
 // work-list order (segment (b, h) after segment, tiles in order) so the issue
@@ -288,7 +190,9 @@ __device__ __forceinline__ int out_dim1(int n, int c) {
   return kFp8 ? 32 * c + 16 + n : 8 * n + 2 * c + 1;
 }
 
-template <typename T, bool kFp8>
+// kScored: the scores and each head's softmax denominator are stored too, for the
+// accumulation of attention weights (kv_scores.cu).
+template <typename T, bool kFp8, bool kScored = false>
 __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const Params p) {
@@ -314,7 +218,7 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
     fence_barrier_init();
   }
   uint32_t err_bits = 0;
-  build_prefix(p, prefix, &err_bits);  // contains __syncthreads
+  build_prefix<kTile>(p, prefix, &err_bits);  // contains __syncthreads
   if (err_bits && threadIdx.x == 0) record_error(p.err, err_bits);
 
   const int64_t total = prefix[p.batch];
@@ -543,6 +447,19 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
           }
         }
       }
+      if constexpr (kScored) {
+        const int64_t pos = static_cast<int64_t>(j) * kTile;
+        const int64_t room = min(static_cast<int64_t>(valid), p.logits_stride - pos);
+        float *lg = p.logits + (static_cast<int64_t>(r.b) * p.hkv * G + r.h * G + g) * p.logits_stride + pos;
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e2 = 0; e2 < 2; ++e2) {
+            const int tok = nt * 8 + 2 * c + e2;
+            if (tok < room && g < G) lg[tok] = sc[nt][e2];
+            if (tok < room && g + 8 < G) lg[8 * p.logits_stride + tok] = sc[nt][2 + e2];
+          }
+      }
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
@@ -650,6 +567,11 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     const bool whole = (t == r.seg_start) && (piece_end == seg_end);
     if (whole) {
+      if constexpr (kScored) {
+        float *lse = p.lse + static_cast<int64_t>(r.b) * p.hkv * G + r.h * G;
+        if (c == 0 && g < G) lse[g] = m0 + log2f(l0);
+        if (c == 0 && g + 8 < G) lse[g + 8] = m1 + log2f(l1);
+      }
       const float inv0 = l0 > 0.f ? vs_cur / l0 : 0.f;
       const float inv1 = l1 > 0.f ? vs_cur / l1 : 0.f;
       T *ob = static_cast<T *>(p.out) + static_cast<int64_t>(r.b) * p.out_sb +
@@ -722,7 +644,7 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
 // of every non-empty slot up to this one).  Warp w merges query-head rows w,
 // w + 4, ... in one pass with a running max, so each piece costs one round of
 // independent loads; lane l owns dims [4l, 4l+4).
-template <typename T>
+template <typename T, bool kScored = false>
 __global__ void __launch_bounds__(128) paged_decode_merge_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t s = blockIdx.x;
@@ -731,12 +653,18 @@ __global__ void __launch_bounds__(128) paged_decode_merge_kernel(const Params p)
   if (job.x < 0) return;
   const int G = p.group;
   const int64_t total = job.w, s_lo = job.z;
+  // Slot t is empty when floor((t + 1) total / nslots) == floor(t total / nslots); the
+  // remainder of t total / nslots is carried along instead of dividing twice a slot.
+  const int64_t step = total % p.nslots, rem_lo = (s_lo * total) % p.nslots;
   for (int row = warp; row < G; row += 4) {
     float m = -INFINITY, l = 0.f;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    int64_t rem = rem_lo;
     for (int64_t t = s_lo; t <= s; ++t) {
-      if (t > s_lo && range_start(t + 1, total, p.nslots) == range_start(t, total, p.nslots))
-        continue;
+      rem += step;
+      const bool crosses = rem >= p.nslots;
+      if (crosses) rem -= p.nslots;
+      if (t > s_lo && total < p.nslots && !crosses) continue;
       const float *pr = p.partials + ((t * 2 + (t == s_lo ? 1 : 0)) * G + row) *
                                          static_cast<int64_t>(kRowFloats);
       const float mt = pr[0], lt = pr[1];
@@ -752,6 +680,8 @@ __global__ void __launch_bounds__(128) paged_decode_merge_kernel(const Params p)
       m = mn;
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (kScored && lane == 0)
+      p.lse[static_cast<int64_t>(job.x) * p.hkv * G + job.y * G + row] = m + log2f(l);
     T *ob = static_cast<T *>(p.out) + static_cast<int64_t>(job.x) * p.out_sb +
             static_cast<int64_t>(job.y * G + row) * p.out_sh + lane * 4;
     *reinterpret_cast<uint2 *>(ob) = make_uint2(Mma<T>::pack(acc[0] * inv, acc[1] * inv),
@@ -813,7 +743,7 @@ size_t workspace_bytes_for(int sms, int group, int warps = Ring<false>::kWarpsPe
   return partial_bytes_for(sms, group, warps) + static_cast<size_t>(sms) * warps * sizeof(int4);
 }
 
-template <typename T, bool kFp8>
+template <typename T, bool kFp8, bool kScored = false>
 int launch(const Params &p0, const CUtensorMap &km, const CUtensorMap &vm, int sms,
            cudaStream_t stream) {
   constexpr int kW = Ring<kFp8>::kWarpsPerCta;
@@ -822,15 +752,15 @@ int launch(const Params &p0, const CUtensorMap &km, const CUtensorMap &vm, int s
   static std::once_flag once;
   static bool ok = false;
   std::call_once(once, [] {
-    ok = cudaFuncSetAttribute(paged_decode_kernel<T, kFp8>,
+    ok = cudaFuncSetAttribute(paged_decode_kernel<T, kFp8, kScored>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                               1024 + kRingBytes + kW * Ring<kFp8>::kStages * 8 +
                                   (kMaxBatch + 1) * sizeof(int32_t)) == cudaSuccess;
   });
   if (!ok) return SLOKV_ERR_CUDA;
-  paged_decode_kernel<T, kFp8><<<sms, kW * 32, smem, stream>>>(km, vm, p0);
+  paged_decode_kernel<T, kFp8, kScored><<<sms, kW * 32, smem, stream>>>(km, vm, p0);
   if (cudaGetLastError() != cudaSuccess) return SLOKV_ERR_CUDA;
-  paged_decode_merge_kernel<T><<<p0.nslots, 128, 0, stream>>>(p0);
+  paged_decode_merge_kernel<T, kScored><<<p0.nslots, 128, 0, stream>>>(p0);
   return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
 }
 
@@ -1022,13 +952,14 @@ int run_decode(bool fp8, void *out, int64_t out_stride_b, int64_t out_stride_h, 
                const int32_t *block_tables, int64_t block_table_stride,
                int32_t max_blocks_per_seq, const int32_t *context_lens, int32_t batch,
                float softmax_scale, int32_t dtype, void *workspace, size_t workspace_bytes,
-               uint32_t *dev_error, void *stream) {
+               uint32_t *dev_error, void *stream, float *logits = nullptr,
+               int64_t logits_stride = 0, float *lse = nullptr) {
   if (batch < 0 || num_blocks <= 0 || block_size <= 0 || num_kv_heads <= 0 || num_q_heads <= 0)
     return SLOKV_ERR_INVALID_ARG;
   if (batch == 0) return SLOKV_OK;
   if (batch > kMaxBatch) return SLOKV_ERR_UNSUPPORTED;
   if (head_dim != kD) return SLOKV_ERR_UNSUPPORTED;
-  const bool f32 = !fp8 && dtype == SLOKV_DTYPE_F32;
+  const bool f32 = !fp8 && !logits && dtype == SLOKV_DTYPE_F32;
   if (dtype != SLOKV_DTYPE_BF16 && dtype != SLOKV_DTYPE_F16 && !f32) return SLOKV_ERR_UNSUPPORTED;
   if (num_q_heads % num_kv_heads) return SLOKV_ERR_INVALID_ARG;
   const int group = num_q_heads / num_kv_heads;
@@ -1096,10 +1027,16 @@ int run_decode(bool fp8, void *out, int64_t out_stride_b, int64_t out_stride_h, 
                                     partial_bytes_for(sms, group, warps));
   p.err = dev_error;
   p.nslots = sms * warps;
+  p.logits = logits;
+  p.lse = lse;
+  p.logits_stride = logits_stride;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (fp8)
     return dtype == SLOKV_DTYPE_BF16 ? launch<__nv_bfloat16, true>(p, km, vm, sms, st)
                                      : launch<__half, true>(p, km, vm, sms, st);
+  if (logits)
+    return dtype == SLOKV_DTYPE_BF16 ? launch<__nv_bfloat16, false, true>(p, km, vm, sms, st)
+                                     : launch<__half, false, true>(p, km, vm, sms, st);
   return dtype == SLOKV_DTYPE_BF16 ? launch<__nv_bfloat16, false>(p, km, vm, sms, st)
                                    : launch<__half, false>(p, km, vm, sms, st);
 }
@@ -1147,6 +1084,28 @@ extern "C" int slokv_paged_decode(void *out, int64_t out_stride_b, int64_t out_s
       k_block_stride, v_block_stride, nullptr, nullptr, num_blocks, block_size, num_q_heads,
       num_kv_heads, head_dim, block_tables, block_table_stride, max_blocks_per_seq,
       context_lens, batch, softmax_scale, dtype, workspace, workspace_bytes, dev_error, stream);
+}
+
+extern "C" int slokv_paged_decode_logits(void *out, int64_t out_stride_b, int64_t out_stride_h,
+                                         const void *q, int64_t q_stride_b, int64_t q_stride_h,
+                                         const void *k_cache, const void *v_cache,
+                                         int64_t k_block_stride, int64_t v_block_stride,
+                                         int32_t num_blocks, int32_t block_size,
+                                         int32_t num_q_heads, int32_t num_kv_heads,
+                                         int32_t head_dim, const int32_t *block_tables,
+                                         int64_t block_table_stride, int32_t max_blocks_per_seq,
+                                         const int32_t *context_lens, int32_t batch,
+                                         float softmax_scale, int32_t dtype, float *logits,
+                                         int64_t logits_stride, float *lse, void *workspace,
+                                         size_t workspace_bytes, uint32_t *dev_error,
+                                         void *stream) {
+  if (batch > 0 && (!logits || !lse || logits_stride <= 0)) return SLOKV_ERR_INVALID_ARG;
+  return slokv::decode::run_decode(
+      false, out, out_stride_b, out_stride_h, q, q_stride_b, q_stride_h, k_cache, v_cache,
+      k_block_stride, v_block_stride, nullptr, nullptr, num_blocks, block_size, num_q_heads,
+      num_kv_heads, head_dim, block_tables, block_table_stride, max_blocks_per_seq,
+      context_lens, batch, softmax_scale, dtype, workspace, workspace_bytes, dev_error, stream,
+      logits, logits_stride, lse);
 }
 
 extern "C" int slokv_paged_decode_fp8(void *out, int64_t out_stride_b, int64_t out_stride_h,
