@@ -10,10 +10,15 @@
 // parameters are its own, so nothing stored before is touched and a page needs no
 // reset when it changes hands.
 //
-// Mapping: half a warp per row of 128 dims, 8 dims a lane: one 16-byte load, a
-// three-step shuffle min / max over the 8 lanes of a group, one 32-bit word of
-// codes stored (the half warp's words are the row's 64 contiguous bytes).  Neighbouring
-// half warps take K and V of one (token, head), then the next head.
+// Append: half a warp per row of 128 dims, 8 dims a lane: one 16-byte load, a three-step
+// shuffle min / max over the 8 lanes of a group, one 32-bit word of codes stored (the half
+// warp's words are the row's 64 contiguous bytes).  A CTA takes 8 tokens of one head, K
+// and V, so its rows are neighbours in the page.  The quotient is a multiplication by
+// 1 / scale, 2^-23 of itself off; where that leaves it within 2^-12 of a border between
+// two codes the lane divides, so the codes are those of the true division.
+//
+// Read-back and widening: eight lanes per row, each with the 8 bytes that hold 8 dims
+// of either group, so that the 16-byte stores of a row are contiguous.
 #include "common.cuh"
 #include "int4_page.cuh"
 
@@ -53,6 +58,34 @@ __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
   }
 }
 
+// Codes of 8 values of a group with minimum m and scale s > 0, the k-th in bits 4k ..
+__device__ __forceinline__ uint32_t encode8(const float (&x)[8], float m, float s) {
+  const float inv = __fdiv_rn(1.f, s);
+  const float magic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
+  uint32_t word = 0;
+  bool near = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = __fsub_rn(x[i], m);
+    const float t = __fmaf_rn(d, inv, magic);
+    const float off = __fmaf_rn(d, inv, -__fsub_rn(t, magic));
+    near |= !(fabsf(off) <= 0.49975586f);  // 0.5 - 2^-12; NaN and infinity too
+    const int c = static_cast<int>(__float_as_uint(t)) - static_cast<int>(__float_as_uint(magic));
+    word |= static_cast<uint32_t>(min(max(c, 0), 15)) << (4 * i);
+  }
+  if (near) {
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = rintf(__fdiv_rn(__fsub_rn(x[i], m), s));
+      word |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
+    }
+  }
+  return word;
+}
+
+constexpr int kTokensPerCta = kRowsPerCta / 2;  // K and V
+
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads)
     kv_append_int4_kernel(const T *__restrict__ key, int64_t key_stride, int64_t key_head,
@@ -62,25 +95,20 @@ __global__ void __launch_bounds__(kThreads)
                           const int32_t *__restrict__ slots, int32_t tokens, int32_t hkv,
                           int32_t block_size, int32_t num_blocks, uint32_t *err) {
   const int lane = threadIdx.x & 31, sub = lane & 15;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 4);
-  const int64_t rows = static_cast<int64_t>(tokens) * hkv * 2;
-  // every lane takes part in the shuffles; `live` guards the memory accesses
-  bool live = row < rows;
-  const bool is_v = row & 1;
-  const int64_t th = row >> 1;
-  const int32_t t = live ? static_cast<int32_t>(th / hkv) : 0;
-  const int32_t h = live ? static_cast<int32_t>(th - static_cast<int64_t>(t) * hkv) : 0;
-  const int32_t slot = live ? __ldg(slots + t) : -1;
-  if (slot < 0 || slot / block_size >= num_blocks) {
-    if (live && slot != -1 && sub == 0) record_error(err, SLOKV_DEVERR_SLOT_RANGE);
-    live = false;
+  // a warp holds K and V of one token: every lane takes part in the shuffles
+  const bool is_v = lane >= 16;
+  const int32_t chunk = blockIdx.x / hkv, h = blockIdx.x - chunk * hkv;
+  const int32_t t = chunk * kTokensPerCta + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  const int32_t slot = __ldg(slots + t);
+  const int32_t blk = slot / block_size, off = slot - blk * block_size;
+  if (slot < 0 || blk >= num_blocks) {
+    if (slot != -1 && lane == 0) record_error(err, SLOKV_DEVERR_SLOT_RANGE);
+    return;
   }
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live) {
-    const T *src = is_v ? value + t * value_stride + h * value_head
-                        : key + t * key_stride + h * key_head;
-    load8<T, kVec>(src + sub * 8, x);
-  }
+  float x[8];
+  const T *src = is_v ? value + t * value_stride + h * value_head : key + t * key_stride + h * key_head;
+  load8<T, kVec>(src + sub * 8, x);
   float mn = x[0], mx = x[0];
   bool bad = false;
 #pragma unroll
@@ -100,16 +128,7 @@ __global__ void __launch_bounds__(kThreads)
   const __nv_bfloat16 mb = __float2bfloat16_rn(mn);
   const float s = __bfloat162float(sb), m = __bfloat162float(mb);
   bad |= !isfinite(s) || !isfinite(m);
-  uint32_t word = 0;
-  if (!bad && s > 0.f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fdiv_rn(__fsub_rn(x[i], m), s));
-      word |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
-    }
-  }
-  if (!live) return;
-  const int32_t blk = slot / block_size, off = slot - blk * block_size;
+  const uint32_t word = !bad && s > 0.f ? encode8(x, m, s) : 0u;
   uint8_t *run = (is_v ? v_cache + blk * v_block_stride : k_cache + blk * k_block_stride) +
                  static_cast<int64_t>(h) * block_size * kRowBytes;
   const int grp = sub >> 3, i = sub & 7;
@@ -122,39 +141,52 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// The 8 values of natural word (group, i) of a row.
-__device__ __forceinline__ void row_values(const uint8_t *run, int32_t off, int grp, int i,
-                                           float (&v)[8]) {
-  const uint32_t w =
-      __ldg(reinterpret_cast<const uint32_t *>(run + code_offset(off) + (2 * i + grp) * 4));
-  const uint32_t pw = __ldg(reinterpret_cast<const uint32_t *>(run + param_offset(off) + 4 * grp));
+constexpr int kWideRows = kThreads / 8;   // rows at a time of the read-back and the widening
+
+// What lane i of eight holds of a row: dims 8i .. 8i + 7 of either group, and both groups'
+// parameters.
+struct Piece {
+  uint2 code, par;
+};
+
+__device__ __forceinline__ Piece load_piece(const uint8_t *run, int32_t off, int i) {
+  return {__ldg(reinterpret_cast<const uint2 *>(run + code_offset(off) + 8 * i)),
+          __ldg(reinterpret_cast<const uint2 *>(run + param_offset(off)))};
+}
+
+__device__ __forceinline__ void piece_values(const Piece &p, int grp, float (&v)[8]) {
+  const uint32_t w = grp ? p.code.y : p.code.x, pw = grp ? p.par.y : p.par.x;
   const float s = scale_of(pw), m = min_of(pw);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = fmaf(s, static_cast<float>((w >> (4 * k)) & 15u), m);
 }
 
-// fp32 values of the rows at `slots` (-1 or outside the pool: zeros), half a warp a row.
+// fp32 values of the rows at `slots` (-1 or outside the pool: zeros).
 __global__ void __launch_bounds__(kThreads)
     int4_decode_kernel(const uint8_t *__restrict__ cache, int64_t block_stride,
                        const int32_t *__restrict__ slots, int32_t tokens, int32_t hkv,
                        int32_t block_size, int32_t num_blocks, float *__restrict__ out,
                        uint32_t *err) {
-  const int sub = threadIdx.x & 15;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 4);
-  if (row >= static_cast<int64_t>(tokens) * hkv) return;
-  const int32_t t = static_cast<int32_t>(row / hkv), h = static_cast<int32_t>(row % hkv);
+  const int i = threadIdx.x & 7;
+  const int32_t chunk = blockIdx.x / hkv, h = blockIdx.x - chunk * hkv;
+  const int32_t t = chunk * kWideRows + (threadIdx.x >> 3);
+  if (t >= tokens) return;
   const int32_t slot = __ldg(slots + t);
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && slot / block_size < num_blocks) {
-    const int32_t blk = slot / block_size;
-    row_values(cache + blk * block_stride + static_cast<int64_t>(h) * block_size * kRowBytes,
-               slot - blk * block_size, sub >> 3, sub & 7, v);
-  } else if (slot != -1 && sub == 0) {
+  const int32_t blk = slot / block_size;
+  Piece p = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+  if (slot >= 0 && blk < num_blocks)
+    p = load_piece(cache + blk * block_stride + static_cast<int64_t>(h) * block_size * kRowBytes,
+                   slot - blk * block_size, i);
+  else if (slot != -1 && i == 0)
     record_error(err, SLOKV_DEVERR_SLOT_RANGE);
+  float *o = out + (static_cast<int64_t>(t) * hkv + h) * kHeadDim + i * 8;
+#pragma unroll
+  for (int grp = 0; grp < 2; ++grp) {
+    float v[8];
+    piece_values(p, grp, v);
+    reinterpret_cast<float4 *>(o + 64 * grp)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(o + 64 * grp)[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
-  float4 *o = reinterpret_cast<float4 *>(out + row * kHeadDim + sub * 8);
-  o[0] = make_float4(v[0], v[1], v[2], v[3]);
-  o[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
 // Widen the cached tokens of a prefill call's rows to bf16 / f16: token t of row r goes to
@@ -189,27 +221,36 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t stride = is_v ? v_block_stride : k_block_stride;
   T *dst = (is_v ? dst_v : dst_k) +
            (static_cast<int64_t>(blockIdx.x) * kWidePage * hkv + h) * kHeadDim;
-  const int sub = threadIdx.x & 15;
-#pragma unroll 4
-  for (int32_t i = threadIdx.x >> 4; i < kWidePage; i += kRowsPerCta) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const int64_t t = t0 + i;
-    if (t < keys) {
-      const int32_t col = static_cast<int32_t>(t / block_size);
-      const int32_t blk = __ldg(tables + r * bt_stride + col);
-      if (blk >= 0 && blk < num_blocks)
-        row_values(cache + blk * stride + static_cast<int64_t>(h) * block_size * kRowBytes,
-                   static_cast<int32_t>(t - static_cast<int64_t>(col) * block_size), sub >> 3,
-                   sub & 7, v);
-      else if (sub == 0)
-        record_error(err, SLOKV_DEVERR_BLOCK_RANGE);
+  const int i = threadIdx.x & 7;
+  constexpr int kSteps = kWidePage / kWideRows;
+  Piece piece[kSteps];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {              // all loads before the first store
+    piece[k] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+    const int64_t t = t0 + k * kWideRows + (threadIdx.x >> 3);
+    if (t >= keys) continue;
+    const int32_t col = static_cast<int32_t>(t) / block_size;
+    const int32_t blk = __ldg(tables + r * bt_stride + col);
+    if (blk >= 0 && blk < num_blocks)
+      piece[k] = load_piece(cache + blk * stride + static_cast<int64_t>(h) * block_size * kRowBytes,
+                            static_cast<int32_t>(t) - col * block_size, i);
+    else if (i == 0)
+      record_error(err, SLOKV_DEVERR_BLOCK_RANGE);
+  }
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    T *o = dst + static_cast<int64_t>(k * kWideRows + (threadIdx.x >> 3)) * hkv * kHeadDim + i * 8;
+#pragma unroll
+    for (int grp = 0; grp < 2; ++grp) {
+      float v[8];
+      piece_values(piece[k], grp, v);
+      uint4 w;
+      w.x = Mma<T>::pack(v[0], v[1]);
+      w.y = Mma<T>::pack(v[2], v[3]);
+      w.z = Mma<T>::pack(v[4], v[5]);
+      w.w = Mma<T>::pack(v[6], v[7]);
+      *reinterpret_cast<uint4 *>(o + 64 * grp) = w;
     }
-    uint4 w;
-    w.x = Mma<T>::pack(v[0], v[1]);
-    w.y = Mma<T>::pack(v[2], v[3]);
-    w.z = Mma<T>::pack(v[4], v[5]);
-    w.w = Mma<T>::pack(v[6], v[7]);
-    *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(i) * hkv * kHeadDim + sub * 8) = w;
   }
 }
 
@@ -248,15 +289,15 @@ extern "C" int slokv_kv_append_int4(const void *key, int64_t key_row_stride,
   const int elem = in_dtype == SLOKV_DTYPE_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & (elem - 1))
     return SLOKV_ERR_ALIGNMENT;
-  const int64_t rows = static_cast<int64_t>(num_tokens) * num_kv_heads * 2;
-  const int64_t ctas = (rows + kRowsPerCta - 1) / kRowsPerCta;
-  if (ctas > 0x7fffffff) return SLOKV_ERR_UNSUPPORTED;
+  const int64_t chunks = (static_cast<int64_t>(num_tokens) + kTokensPerCta - 1) / kTokensPerCta;
+  if (chunks * num_kv_heads > 0x7fffffff) return SLOKV_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(chunks * num_kv_heads);
   const bool vec = vec_ok(key, key_row_stride, key_head_stride, elem) &&
                    vec_ok(value, value_row_stride, value_head_stride, elem);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto kernel, auto tag) {
     using T = decltype(tag);
-    kernel<<<static_cast<unsigned>(ctas), kThreads, 0, st>>>(
+    kernel<<<grid, kThreads, 0, st>>>(
         static_cast<const T *>(key), key_row_stride, key_head_stride,
         static_cast<const T *>(value), value_row_stride, value_head_stride,
         static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_block_stride,
@@ -287,10 +328,9 @@ extern "C" int slokv_int4_decode(const void *cache, int64_t block_stride,
   if (!pool_ok(cache, block_stride, num_kv_heads, block_size) ||
       (reinterpret_cast<uintptr_t>(out) & 15u))
     return SLOKV_ERR_ALIGNMENT;
-  const int64_t rows = static_cast<int64_t>(num_tokens) * num_kv_heads;
-  const int64_t ctas = (rows + kRowsPerCta - 1) / kRowsPerCta;
-  if (ctas > 0x7fffffff) return SLOKV_ERR_UNSUPPORTED;
-  int4_decode_kernel<<<static_cast<unsigned>(ctas), kThreads, 0,
+  const int64_t chunks = (static_cast<int64_t>(num_tokens) + kWideRows - 1) / kWideRows;
+  if (chunks * num_kv_heads > 0x7fffffff) return SLOKV_ERR_UNSUPPORTED;
+  int4_decode_kernel<<<static_cast<unsigned>(chunks * num_kv_heads), kThreads, 0,
                        static_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint8_t *>(cache), block_stride, slot_mapping, num_tokens, num_kv_heads,
       block_size, num_blocks, out, dev_error);

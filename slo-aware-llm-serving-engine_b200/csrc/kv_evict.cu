@@ -10,9 +10,10 @@
 //
 // kv_evict_select_kernel, one CTA per (b, h): the scores become unsigned keys of the
 // same order (kept in shared memory up to kSmemKeys tokens, else read again through
-// L2), a radix select over 4 x 8 bits finds the key of the last token that stays, and
-// three ordered passes with warp votes (each warp owns a contiguous piece) rank ties,
-// holes and moved tokens.  It writes the move list and compacts the score row.
+// L2), a radix select of at most 4 x 8 bits finds the key of the last token that stays, and
+// warp votes turn the row into 32-token words (each warp owns a contiguous piece), from
+// which ties, holes and moved tokens are ranked.  It writes the move list and compacts
+// the score row.
 // kv_evict_move_kernel then copies the rows, spread over the whole GPU.
 #include "common.cuh"
 #include "int4_page.cuh"
@@ -22,12 +23,11 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kSmemKeys = 8192;     // 32 KiB: four CTAs a multiprocessor
-constexpr int kCopies = 8;          // histogram copies, so that equal keys collide less
+constexpr int kSmemKeys = 8192;     // 32 KiB
+constexpr int kCopies = 4;          // histogram copies, so that equal keys collide less
 constexpr int kMoveThreads = 256;
-constexpr int kMovesPerCta = 64;
+constexpr int kMovesPerWarp = 8;
+constexpr int kMovesPerCta = kMoveThreads / 32 * kMovesPerWarp;
 
 struct EvictParams {
   uint8_t *k_cache, *v_cache;
@@ -57,10 +57,12 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictParams p) {
+  constexpr int kWarps = kThreads / 32;
   extern __shared__ uint32_t keys[];
   __shared__ uint32_t hist[kCopies][256];
-  __shared__ uint32_t sh_prefix, sh_left;
+  __shared__ uint32_t sh_prefix, sh_left, sh_done;
   __shared__ uint32_t piece[3][kWarps];   // ties, holes, moved tokens of each warp's piece
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv;
@@ -90,7 +92,8 @@ __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictPa
 
   // ---- the need-th largest key: 8 bits a pass, most significant first ----
   uint32_t prefix = 0, left = need;             // left: places for keys that share the prefix
-  for (int shift = 24; need && shift >= 0; shift -= 8) {
+  bool done = need == 0;                        // every key that shares the prefix stays
+  for (int shift = 24; !done && shift >= 0; shift -= 8) {
     for (int i = tid; i < kCopies * 256; i += kThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
     for (int32_t t = tid; t < old; t += kThreads) {
@@ -121,46 +124,85 @@ __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictPa
         while (rest > bin[i]) rest -= bin[i++];
         sh_prefix = prefix | (static_cast<uint32_t>(255 - 8 * lane - i) << shift);
         sh_left = rest;
+        sh_done = rest == bin[i];
       }
     }
     __syncthreads();
     prefix = sh_prefix;
     left = sh_left;
+    done = sh_done;
   }
   __syncthreads();                              // the keys are in place (need == 0: no pass ran)
 
-  // ---- ordered ranks: warp w owns tokens [lo, hi) ----
-  const int32_t per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int32_t lo = min(n, warp * per), hi = min(n, lo + per);
+  // ---- ordered ranks, 32 tokens to a word; warp w owns the words [lo, hi) ----
+  // A key of at least `least` stays, and of the holders of the key `prefix` the first `left`.
+  const uint32_t least = need == 0 ? 0xffffffffu : done ? prefix : prefix + 1;
+  const bool ties_exist = !done;
+  const int32_t words = (n + 31) / 32, per = (words + kWarps - 1) / kWarps;
+  const int32_t lo = min(words, warp * per), hi = min(words, lo + per);
   const uint32_t below = (1u << lane) - 1u;
-  uint32_t ties = 0;
-  if (need)
-    for (int32_t t0 = lo; t0 < hi; t0 += 32) {
-      const int32_t t = t0 + lane;
-      ties += __popc(__ballot_sync(0xffffffffu, t < min(hi, old) && key(t) == prefix));
+  // Lane i gets what the tokens of word w0 + i are: certain to stay, or ties.
+  uint32_t sure = 0, tie = 0;
+  auto classify = [&](int32_t w0) {
+    sure = tie = 0;
+    const int32_t stop = min(32, hi - w0);
+    for (int32_t i = 0; i < stop; ++i) {
+      const int32_t t = (w0 + i) * 32 + lane;
+      const uint32_t k = t < old ? key(t) : 0u;
+      const uint32_t a = __ballot_sync(0xffffffffu, t < n && (t >= old || k >= least));
+      const uint32_t b = __ballot_sync(0xffffffffu, ties_exist && t < old && k == prefix);
+      if (lane == i) {
+        sure = a;
+        tie = b;
+      }
     }
+  };
+  auto inclusive = [&](uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += x;
+    }
+    return v;
+  };
+  // Holes and moved tokens of lane i's word, given the ties before the group of words.
+  uint32_t hole = 0, mover = 0;
+  auto place = [&](int32_t w0, uint32_t &tie_base) {
+    const uint32_t upto = inclusive(__popc(tie));
+    const uint32_t before = tie_base + upto - __popc(tie);
+    uint32_t some = tie;
+    const uint32_t room = before < left ? left - before : 0u;
+    if (room == 0) some = 0;
+    while (__popc(some) > room) some &= ~(0x80000000u >> __clz(some));  // one word at most
+    tie_base += __shfl_sync(0xffffffffu, upto, 31);
+    const int32_t t0 = (w0 + lane) * 32;
+    auto mask_below = [&](int32_t limit) {
+      return limit >= t0 + 32 ? 0xffffffffu : limit <= t0 ? 0u : (1u << (limit - t0)) - 1u;
+    };
+    const bool mine = w0 + lane < hi;
+    const uint32_t stays = sure | some, under = mask_below(p.keep);
+    hole = mine ? ~stays & mask_below(n) & under : 0u;
+    mover = mine ? stays & ~under : 0u;
+  };
+  const bool single = per <= 32;                // one group of words: classified once
+  uint32_t ties = 0;
+  for (int32_t w0 = lo; w0 < hi; w0 += 32) {
+    classify(w0);
+    ties += __shfl_sync(0xffffffffu, inclusive(__popc(tie)), 31);
+  }
   if (lane == 0) piece[0][warp] = ties;
   __syncthreads();
   uint32_t tie_base = 0;
   for (int w = 0; w < warp; ++w) tie_base += piece[0][w];
-  // kept[t]: recent, above the threshold key, or one of its first `left` holders
-  auto kept_at = [&](int32_t t, uint32_t &base) {
-    const bool in = t < hi, cand = in && t < old && need;
-    const uint32_t k = cand ? key(t) : 0u;
-    const bool tie = cand && k == prefix;
-    const uint32_t votes = __ballot_sync(0xffffffffu, tie);
-    const bool keep = in && (t >= old || (cand && k > prefix) ||
-                             (tie && base + __popc(votes & below) < left));
-    base += __popc(votes);
-    return keep;
-  };
   uint32_t base = tie_base, holes = 0, moved = 0;
-  for (int32_t t0 = lo; t0 < hi; t0 += 32) {
-    const int32_t t = t0 + lane;
-    const bool k = kept_at(t, base);
-    holes += __popc(__ballot_sync(0xffffffffu, t < hi && t < p.keep && !k));
-    moved += __popc(__ballot_sync(0xffffffffu, t >= p.keep && k));
+  for (int32_t w0 = lo; w0 < hi; w0 += 32) {
+    if (!single) classify(w0);
+    place(w0, base);
+    holes += __popc(hole);
+    moved += __popc(mover);
   }
+  holes = __reduce_add_sync(0xffffffffu, holes);
+  moved = __reduce_add_sync(0xffffffffu, moved);
   if (lane == 0) {
     piece[1][warp] = holes;
     piece[2][warp] = moved;
@@ -177,15 +219,20 @@ __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictPa
   int32_t *dst = p.moves + static_cast<int64_t>(blockIdx.x) * 2 * p.max_moves;
   int32_t *src = dst + p.max_moves;
   base = tie_base;
-  for (int32_t t0 = lo; t0 < hi; t0 += 32) {
-    const int32_t t = t0 + lane;
-    const bool k = kept_at(t, base);
-    const bool hole = t < hi && t < p.keep && !k, mover = t >= p.keep && k;
-    const uint32_t hv = __ballot_sync(0xffffffffu, hole), mv = __ballot_sync(0xffffffffu, mover);
-    if (hole) dst[hole_at + __popc(hv & below)] = t;
-    if (mover) src[move_at + __popc(mv & below)] = t;
-    hole_at += __popc(hv);
-    move_at += __popc(mv);
+  for (int32_t w0 = lo; w0 < hi; w0 += 32) {
+    if (!single) {
+      classify(w0);
+      place(w0, base);
+    }
+    const int32_t stop = min(32, hi - w0);
+    for (int32_t i = 0; i < stop; ++i) {
+      const uint32_t hv = __shfl_sync(0xffffffffu, hole, i), mv = __shfl_sync(0xffffffffu, mover, i);
+      const int32_t t = (w0 + i) * 32 + lane;
+      if ((hv >> lane) & 1u) dst[hole_at + __popc(hv & below)] = t;
+      if ((mv >> lane) & 1u) src[move_at + __popc(mv & below)] = t;
+      hole_at += __popc(hv);
+      move_at += __popc(mv);
+    }
   }
   if (tid == 0) p.counts[blockIdx.x] = static_cast<int32_t>(total);
   __syncthreads();
@@ -205,41 +252,69 @@ __global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const Evict
   const int32_t *dst = p.moves + static_cast<int64_t>(pair) * 2 * p.max_moves;
   const int32_t *src = dst + p.max_moves;
   const int32_t *table = p.tables + static_cast<int64_t>(b) * p.bt_stride;
-  const int32_t stop = min(count, static_cast<int32_t>(blockIdx.y + 1) * kMovesPerCta);
-  for (int32_t i = blockIdx.y * kMovesPerCta + warp; i < stop; i += kMoveThreads / 32) {
-    const int32_t to = __ldg(dst + i), from = __ldg(src + i);
-    const int32_t tb = __ldg(table + to / p.block_size), fb = __ldg(table + from / p.block_size);
+  // lanes 0 .. 7 look up the warp's moves, then all their rows are loaded before any is stored
+  const int32_t first = blockIdx.y * kMovesPerCta + warp * kMovesPerWarp;
+  if (first >= count) return;
+  int32_t tb = -1, fb = 0, to_off = 0, from_off = 0;
+  if (lane < kMovesPerWarp && first + lane < count) {
+    const int32_t to = __ldg(dst + first + lane), from = __ldg(src + first + lane);
+    const int32_t to_page = to / p.block_size, from_page = from / p.block_size;
+    tb = __ldg(table + to_page);
+    fb = __ldg(table + from_page);
+    to_off = to - to_page * p.block_size;
+    from_off = from - from_page * p.block_size;
     if (tb < 0 || tb >= p.num_blocks || fb < 0 || fb >= p.num_blocks) {
-      if (lane == 0) record_error(p.err, SLOKV_DEVERR_BLOCK_RANGE);
-      continue;
+      record_error(p.err, SLOKV_DEVERR_BLOCK_RANGE);
+      tb = -1;
     }
-    const int32_t to_off = to % p.block_size, from_off = from % p.block_size;
-    if (p.row_bytes) {
-      const int64_t head = static_cast<int64_t>(h) * p.row_bytes;
-      const int64_t token = static_cast<int64_t>(p.hkv) * p.row_bytes;
-      const int half = p.row_bytes / 16;        // 16-byte pieces of a row; K's first, then V's
-      for (int c = lane; c < 2 * half; c += 32) {
-        const bool v = c >= half;
-        uint8_t *cache = v ? p.v_cache : p.k_cache;
-        const int64_t bs = v ? p.v_bs : p.k_bs, at = head + (v ? c - half : c) * 16;
-        const uint4 w = *reinterpret_cast<const uint4 *>(cache + fb * bs + from_off * token + at);
-        *reinterpret_cast<uint4 *>(cache + tb * bs + to_off * token + at) = w;
+  }
+  if (p.row_bytes) {
+    const int64_t head = static_cast<int64_t>(h) * p.row_bytes;
+    const int64_t token = static_cast<int64_t>(p.hkv) * p.row_bytes;
+    const int half = p.row_bytes / 16;          // 16-byte pieces of a row; K's first, then V's
+    for (int c = lane; c < 2 * half; c += 32) {  // 16 or 32 pieces a side: all lanes alike
+      uint8_t *cache = c >= half ? p.v_cache : p.k_cache;
+      const int64_t bs = c >= half ? p.v_bs : p.k_bs;
+      const int64_t at = head + (c >= half ? c - half : c) * 16;
+      uint4 w[kMovesPerWarp];
+#pragma unroll
+      for (int i = 0; i < kMovesPerWarp; ++i) {
+        const int32_t t = __shfl_sync(0xffffffffu, tb, i), f = __shfl_sync(0xffffffffu, fb, i);
+        const int32_t fo = __shfl_sync(0xffffffffu, from_off, i);
+        if (t >= 0) w[i] = *reinterpret_cast<const uint4 *>(cache + f * bs + fo * token + at);
       }
-    } else if (lane < 10) {                     // 5 lanes a side: 4 x 16 B of codes, 8 B of parameters
-      const bool v = lane >= 5;
-      const int c = v ? lane - 5 : lane;
-      uint8_t *cache = v ? p.v_cache : p.k_cache;
-      const int64_t bs = v ? p.v_bs : p.k_bs;
-      const int64_t head = static_cast<int64_t>(h) * p.block_size * kRowBytes;
-      const uint8_t *f = cache + fb * bs + head;
-      uint8_t *t = cache + tb * bs + head;
-      if (c < 4)
-        *reinterpret_cast<uint4 *>(t + code_offset(to_off) + 16 * c) =
-            *reinterpret_cast<const uint4 *>(f + code_offset(from_off) + 16 * c);
-      else
-        *reinterpret_cast<uint2 *>(t + param_offset(to_off)) =
-            *reinterpret_cast<const uint2 *>(f + param_offset(from_off));
+#pragma unroll
+      for (int i = 0; i < kMovesPerWarp; ++i) {
+        const int32_t t = __shfl_sync(0xffffffffu, tb, i), o = __shfl_sync(0xffffffffu, to_off, i);
+        if (t >= 0) *reinterpret_cast<uint4 *>(cache + t * bs + o * token + at) = w[i];
+      }
     }
+  } else {
+    // a 4-bit row is 9 pieces of 8 bytes a side: the lanes take (move, piece) pairs
+    const int64_t head = static_cast<int64_t>(h) * p.block_size * kRowBytes;
+    constexpr int kPieces = 18, kSteps = (kMovesPerWarp * kPieces + 31) / 32;
+    uint2 w[kSteps];
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int item = lane + 32 * k, i = item / kPieces, c = item % kPieces;
+        const int32_t t = __shfl_sync(0xffffffffu, tb, i & 7), f = __shfl_sync(0xffffffffu, fb, i & 7);
+        const int32_t to = __shfl_sync(0xffffffffu, to_off, i & 7);
+        const int32_t fo = __shfl_sync(0xffffffffu, from_off, i & 7);
+        if (i >= kMovesPerWarp || t < 0) continue;
+        const bool v = c >= 9;
+        const int q = v ? c - 9 : c;
+        uint8_t *cache = (v ? p.v_cache : p.k_cache) + head;
+        const int64_t bs = v ? p.v_bs : p.k_bs;
+        const int32_t off = pass ? to : fo;
+        uint2 *at = reinterpret_cast<uint2 *>(cache + (pass ? t : f) * bs +
+                                              (q < 8 ? code_offset(off) + 8 * q : param_offset(off)));
+        if (pass)
+          *at = w[k];
+        else
+          w[k] = *at;
+      }
   }
 }
 
@@ -328,7 +403,12 @@ extern "C" int slokv_kv_evict(void *k_cache, void *v_cache, int64_t k_block_stri
   p.err = dev_error;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t smem = sizeof(uint32_t) * (cap < kSmemKeys ? cap : kSmemKeys);
-  kv_evict_select_kernel<<<static_cast<unsigned>(pairs), kThreads, smem, st>>>(p);
+  // 256 threads: eight CTAs a multiprocessor hide each other's barriers (128 x 8 pairs of
+  // 2304 tokens: 19 us, 42 with 512); long rows, which few pairs have, take 1024.
+  if (cap <= kSmemKeys)
+    kv_evict_select_kernel<256><<<static_cast<unsigned>(pairs), 256, smem, st>>>(p);
+  else
+    kv_evict_select_kernel<1024><<<static_cast<unsigned>(pairs), 1024, smem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SLOKV_ERR_CUDA;
   if (most == 0) return SLOKV_OK;
   const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(chunks));

@@ -659,25 +659,46 @@ __global__ void __launch_bounds__(128) paged_decode_merge_kernel(const Params p)
   for (int row = warp; row < G; row += 4) {
     float m = -INFINITY, l = 0.f;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    int64_t rem = rem_lo;
-    for (int64_t t = s_lo; t <= s; ++t) {
-      rem += step;
-      const bool crosses = rem >= p.nslots;
-      if (crosses) rem -= p.nslots;
-      if (t > s_lo && total < p.nslots && !crosses) continue;
-      const float *pr = p.partials + ((t * 2 + (t == s_lo ? 1 : 0)) * G + row) *
-                                         static_cast<int64_t>(kRowFloats);
-      const float mt = pr[0], lt = pr[1];
-      const float4 v = *reinterpret_cast<const float4 *>(pr + kAccOff + lane * 4);
-      const float mn = fmaxf(m, mt);
-      const float a = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-      const float b = mt == -INFINITY ? 0.f : fast_exp2(mt - mn);
-      l = l * a + lt * b;
-      acc[0] = acc[0] * a + v.x * b;
-      acc[1] = acc[1] * a + v.y * b;
-      acc[2] = acc[2] * a + v.z * b;
-      acc[3] = acc[3] * a + v.w * b;
-      m = mn;
+    int64_t rem = rem_lo, t = s_lo;
+    while (t <= s) {
+      // the next four non-empty slots, all loaded before the first is combined
+      const float *at[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        at[i] = nullptr;
+        while (t <= s && !at[i]) {
+          rem += step;
+          const bool crosses = rem >= p.nslots;
+          if (crosses) rem -= p.nslots;
+          if (t == s_lo || total >= p.nslots || crosses)
+            at[i] = p.partials + ((t * 2 + (t == s_lo ? 1 : 0)) * G + row) *
+                                     static_cast<int64_t>(kRowFloats);
+          ++t;
+        }
+      }
+      float2 ml[4];
+      float4 vv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at[i]) {
+          ml[i] = *reinterpret_cast<const float2 *>(at[i]);
+          vv[i] = *reinterpret_cast<const float4 *>(at[i] + kAccOff + lane * 4);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at[i]) {
+          const float mt = ml[i].x, lt = ml[i].y;
+          const float4 v = vv[i];
+          const float mn = fmaxf(m, mt);
+          const float a = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+          const float b = mt == -INFINITY ? 0.f : fast_exp2(mt - mn);
+          l = l * a + lt * b;
+          acc[0] = acc[0] * a + v.x * b;
+          acc[1] = acc[1] * a + v.y * b;
+          acc[2] = acc[2] * a + v.z * b;
+          acc[3] = acc[3] * a + v.w * b;
+          m = mn;
+        }
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
     if (kScored && lane == 0)

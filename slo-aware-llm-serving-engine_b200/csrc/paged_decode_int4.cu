@@ -8,6 +8,9 @@
 // the 8 x 8 score tile and to the probabilities instead of to the 128 dims: that is
 // 4 FMAs a score instead of 64 a token, and no 4-bit value is ever rounded.
 //
+// The minimum's term of the scores is one bf16 MMA for 16 tokens: the parameter words are its
+// A operand as they lie in the page.
+//
 // QK^T (m16n8k16, f16, S^T = K q^T: A = K codes, 16 tokens; B = q, 8 heads).  A 4-bit code
 // in bits 0-3 of an f16 is the subnormal c 2^-24, in bits 4-7 it is 16 c 2^-24: two masks
 // and one shift turn a word of 8 codes into four f16x2 operands, exactly.  q rows are
@@ -19,11 +22,12 @@
 // score and output columns are the same two heads.  movmatrix turns the score tile into
 // the B operand; a prmt pairs the codes of two tokens, then the same masks apply.  The
 // probabilities carry the V scale, r = f16(p s_g) (half a step is 2^-11, an eighth of
-// a bf16 output's):
+// a bf16 output's), out = sum_t r c + sum_t p m.  For f16 outputs, which round as finely
+// as r does,
 //   out = sum_t r (c - 8) + sum_t p (m + 8 s)
 // with sum_t 8 r from one more MMA with a constant A, so that the rounding of r meets
-// c - 8 instead of c.  f16 has 5 exponent bits and the scales' range is fp32's:
-// the reference that the scores are exponentiated against is not the running maximum
+// c - 8 instead of c: 3.3e-4 instead of 5e-4 off in all, for 2 % of the time.  f16 has 5
+// exponent bits and the scales' range is fp32's: the reference that the scores are exponentiated against is not the running maximum
 // but lies 15 - ceil(log2 max(s, |m|)) below it, the maximum over the tokens seen so
 // far.  r is then at most 2^15 and keeps its 11 bits down to 2^-29 of the largest value;
 // the sum of p is taken against the same reference, so the quotient does not see it.
@@ -38,7 +42,7 @@
 #include "decode_worklist.cuh"
 #include "int4_page.cuh"
 
-#include <mutex>
+#include <type_traits>
 
 namespace slokv {
 namespace decode4 {
@@ -100,6 +104,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 
 // Shared-memory loads as plain C++, which the compiler may schedule between the waits.
 __device__ __forceinline__ uint4 lds128(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
+__device__ __forceinline__ uint32_t lds32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 __device__ __forceinline__ uint2 lds64(const uint8_t *p) { return *reinterpret_cast<const uint2 *>(p); }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
@@ -124,6 +129,21 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32
       "{%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// x in the high half as the bf16 nearest to it; x becomes what that leaves.
+__device__ __forceinline__ uint32_t split_bf16(float &x) {
+  const uint32_t hi = static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x))) << 16;
+  x -= __uint_as_float(hi);
+  return hi;
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
@@ -317,6 +337,7 @@ template <typename T, int kN, bool kScored>
 __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel(const Params p) {
   using MO = Mma<T>;
   constexpr int kWarps = warps_of(kN), kRingBytes = ring_bytes(kWarps);
+  constexpr bool kCentre = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
   uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -394,7 +415,10 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
     // w).  k-step 4 grp + 2 half takes the nibbles (0, 4), (2, 6) of the word, k-step + 1
     // the nibbles (1, 5), (3, 7), which the masks leave 16 times larger.
     uint32_t qb[kN][8][2];
-    float qsum[kN][2][2];   // [rr][group][e]: sum of the group's q of head 8 rr + 2 c + e
+    // B of the minimum's MMA: its A holds a token's (scale, minimum) words as they are, k = 2c
+    // the scale and k = 2c + 1 the minimum of group c & 1, so B has zeros against the scales
+    // and, against the minima, the group's sum of q in three bf16 pieces (24 bits).
+    uint32_t qm[kN][2];
     float unscale[kN][2];   // accumulator unit -> log2-domain score, of the same heads
 #pragma unroll
     for (int rr = 0; rr < kN; ++rr) {
@@ -427,6 +451,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
                              1.17549435e-38f);
       unscale[rr][0] = __shfl_sync(0xffffffffu, un, 8 * c);
       unscale[rr][1] = __shfl_sync(0xffffffffu, un, 8 * c + 4);
+      float qsum[2];
 #pragma unroll
       for (int grp = 0; grp < 2; ++grp) {
         float sum = 0.f;
@@ -444,10 +469,12 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= 5.9604644775390625e-8f;  // 2^-24: the unit of the codes
-        qsum[rr][grp][0] = __shfl_sync(0xffffffffu, sum, 8 * c);
-        qsum[rr][grp][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+        qsum[grp] = sum * 5.9604644775390625e-8f;  // 2^-24: the unit of the codes
       }
+      float rest = c & 1 ? qsum[1] : qsum[0];
+      const uint32_t q_hi = split_bf16(rest), q_mid = split_bf16(rest), q_lo = split_bf16(rest);
+      qm[rr][0] = c < 2 ? q_hi : q_mid;
+      qm[rr][1] = c < 2 ? q_lo : 0u;
     }
 
     // out^T accumulators: o[rr][4 grp + k][x] is dim 64 grp + 8 g + k (+ 4 for x >= 2) of head
@@ -524,18 +551,21 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
                       h1 & 0x00f000f0u, qb[rr][ks + 1][0], qb[rr][ks + 1][1]);
             }
           }
+        const uint32_t mw0 = lds32(kb + kParamOff + (16 * i + tok_k) * 8 + (c & 1) * 4);
+        const uint32_t mw1 = lds32(kb + kParamOff + (16 * i + 8 + tok_k) * 8 + (c & 1) * 4);
+#pragma unroll
+        for (int rr = 0; rr < kN; ++rr)
+          mma_bf16_first(sc[rr][i], mw0, mw1, mw0, mw1, qm[rr][0], qm[rr][1]);
 #pragma unroll
         for (int row = 0; row < 2; ++row) {
           const uint2 pw = lds64(kb + kParamOff + (16 * i + 8 * row + tok_k) * 8);
-          const float s0 = scale_of(pw.x), m0 = min_of(pw.x), s1 = scale_of(pw.y), m1 = min_of(pw.y);
+          const float s0 = scale_of(pw.x), s1 = scale_of(pw.y);
 #pragma unroll
           for (int rr = 0; rr < kN; ++rr)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-              sc[rr][i][2 * row + x] =
-                  fmaf(s0, acc[rr][0][2 * row + x],
-                       fmaf(s1, acc[rr][1][2 * row + x],
-                            fmaf(m0, qsum[rr][0][x], m1 * qsum[rr][1][x])));
+              sc[rr][i][2 * row + x] = fmaf(s0, acc[rr][0][2 * row + x],
+                                            fmaf(s1, acc[rr][1][2 * row + x], sc[rr][i][2 * row + x]));
         }
       }
       if (valid < kTile) {
@@ -571,17 +601,20 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
 
       // ---- online softmax ----
       {
-        // positive floats order as their bits; NaN (above infinity's bits) does not count
+        // positive bf16 order as their bits, and both halves of a word count
         const uint2 p0 = lds64(vb + kParamOff + lane * 8), p1 = lds64(vb + kParamOff + (lane + 32) * 8);
-        uint32_t top = 0;
+        const uint32_t abs2 = 0x7fff7fffu;
+        uint32_t top = __vmaxu2(__vmaxu2(p0.x & abs2, p0.y & abs2), __vmaxu2(p1.x & abs2, p1.y & abs2));
+        top = __reduce_max_sync(0xffffffffu, max(top >> 16, top & 0xffffu));
+        if (top >= 0x7f80u) {  // NaN parameters do not count
+          const uint32_t w[4] = {p0.x & abs2, p0.y & abs2, p1.x & abs2, p1.y & abs2};
+          top = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w = i == 0 ? p0.x : i == 1 ? p0.y : i == 2 ? p1.x : p1.y;
-          const uint32_t sb = w << 16, mb = w & 0x7fff0000u;
-          if (sb < 0x7f800000u) top = max(top, max(sb, mb));
+          for (int i = 0; i < 4; ++i)
+            if ((w[i] & 0xffffu) < 0x7f80u) top = max(top, max(w[i] >> 16, w[i] & 0xffffu));
+          top = __reduce_max_sync(0xffffffffu, top);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        sexp = max(sexp, static_cast<int>(top >> 23) - 126);
+        sexp = max(sexp, static_cast<int>(top >> 7) - 126);
       }
       const float under = static_cast<float>(15 - sexp);
       bool moved = false;
@@ -631,7 +664,8 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
         for (int row = 0; row < 2; ++row) {
           const uint2 pw = lds64(vb + kParamOff + (16 * i + 8 * row + tok_k) * 8);
           const float s0 = scale_of(pw.x), s1 = scale_of(pw.y);
-          const float z0 = fmaf(8.f, s0, min_of(pw.x)), z1 = fmaf(8.f, s1, min_of(pw.y));
+          const float z0 = kCentre ? fmaf(8.f, s0, min_of(pw.x)) : min_of(pw.x);
+          const float z1 = kCentre ? fmaf(8.f, s1, min_of(pw.y)) : min_of(pw.y);
 #pragma unroll
           for (int rr = 0; rr < kN; ++rr) {
             float pr[2];
@@ -666,7 +700,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
                       (lo1 >> sh) & mask, (hi1 >> sh) & mask, pb[rr][grp][0], pb[rr][grp][1]);
           }
 #pragma unroll
-          for (int rr = 0; rr < kN; ++rr)
+          for (int rr = 0; kCentre && rr < kN; ++rr)
             mma_f16(osum[rr][grp], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u,
                     pb[rr][grp][0], pb[rr][grp][1]);
         }
@@ -711,7 +745,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
           // 2^24 undoes the codes' unit, 2^20 that of the codes 16 times larger
-          const float z = fmaf(-16777216.f, osum[rr][grp][x], vz[rr][grp][x]);
+          const float z = kCentre ? fmaf(-16777216.f, osum[rr][grp][x], vz[rr][grp][x]) : vz[rr][grp][x];
           float v[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
