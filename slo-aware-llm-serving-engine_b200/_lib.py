@@ -215,6 +215,35 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The stream's handle without a Stream object around it (0.1 us instead of 2.3 us).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+class on_device:
+    """Make `device` current for a launch and give its current stream's handle:
+    `with on_device(dev) as stream`.  A launch goes to the current device, whatever
+    device its tensors and stream belong to."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.index is None:
+            self.index = self.before
+        elif self.index != self.before:
+            torch.cuda.set_device(self.index)
+        if _raw_stream is not None:
+            return _raw_stream(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return DTYPE_BF16

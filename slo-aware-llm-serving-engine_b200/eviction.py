@@ -21,40 +21,62 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import SlokvError, buffers, check, lib, require_cuda, stream_ptr
+from ._lib import SlokvError, buffers, check, lib, on_device, require_cuda
 from .kvcache import _i32_contig
-from .kvcache_int4 import (HEAD_DIM, _block_stride, _decode_int4, check_decode_args,
-                           int4_geometry, is_int4_cache)
+from .kvcache_int4 import (HEAD_DIM, check_decode_args, decode_int4_workspace_bytes, int4_geometry,
+                           is_int4_cache, launch_decode_int4)
 
 
 def _check_scores(scores, score_rows, batch, num_kv_heads):
-    if scores.dim() != 3 or scores.dtype != torch.float32 or scores.stride(-1) != 1:
-        raise SlokvError("scores must be fp32 [rows, num_kv_heads, width] with a contiguous last "
-                         "dim")
-    if scores.shape[1] != num_kv_heads:
-        raise SlokvError(f"scores have {scores.shape[1]} KV heads, the pool {num_kv_heads}")
+    """(rows, width, row stride, head stride, score_rows' address) of a score table."""
+    if scores.dim() != 3 or scores.dtype != torch.float32:
+        raise SlokvError("scores must be fp32 [rows, num_kv_heads, width]")
+    rows, heads, width = scores.shape
+    row, head, one = scores.stride()
+    if one != 1:
+        raise SlokvError("scores need a contiguous last dimension")
+    if heads != num_kv_heads:
+        raise SlokvError(f"scores have {heads} KV heads, the pool {num_kv_heads}")
     if score_rows is None:
-        if scores.shape[0] < batch:
+        if rows < batch:
             raise SlokvError("scores have fewer rows than the batch")
-    else:
-        _i32_contig("score_rows", score_rows)
-        if score_rows.numel() < batch:
-            raise SlokvError("score_rows has fewer entries than the batch")
+        return rows, width, row, head, None
+    _i32_contig("score_rows", score_rows)
+    if score_rows.numel() < batch:
+        raise SlokvError("score_rows has fewer entries than the batch")
+    return rows, width, row, head, score_rows.data_ptr()
 
 
 def _dense_geometry(k_cache, v_cache, dtypes):
-    """(num_blocks, block_size, num_kv_heads) of an unquantised pool, checked."""
+    """(num_blocks, block_size, num_kv_heads, K and V block strides in elements) of an
+    unquantised pool, checked."""
     if k_cache.dim() != 4 or k_cache.shape[3] != HEAD_DIM or v_cache.shape != k_cache.shape:
         raise SlokvError(f"k_cache / v_cache must be [num_blocks, block_size, Hkv, {HEAD_DIM}] of "
                          "one shape")
     if k_cache.dtype not in dtypes or v_cache.dtype != k_cache.dtype:
-        raise SlokvError(f"k_cache / v_cache must both be one of {dtypes} (FP8 pools are not "
+        raise SlokvError(f"k_cache / v_cache must both be one of {list(dtypes)} (FP8 pools are not "
                          "supported)")
     NB, bs, Hkv, D = k_cache.shape
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.stride(3) != 1 or c.stride(2) != D or c.stride(1) != Hkv * D:
-            raise SlokvError(f"{name} blocks must be contiguous [block_size, Hkv, D]")
-    return NB, bs, Hkv
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if ks[1:] != (Hkv * D, D, 1) or vs[1:] != (Hkv * D, D, 1):
+        raise SlokvError("k_cache / v_cache blocks must be contiguous [block_size, Hkv, D]")
+    return NB, bs, Hkv, ks[0], vs[0]
+
+
+_DECODE_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_EVICT_DTYPES = {**_DECODE_DTYPES, torch.float32: _lib.DTYPE_F32}
+_workspace_bytes = {}   # (device, Hq, Hkv) -> bytes of the bf16 / f16 decode
+
+
+def _decode_workspace_bytes(index, num_q_heads, num_kv_heads):
+    key = (index, num_q_heads, num_kv_heads)
+    n = _workspace_bytes.get(key)
+    if n is None:
+        n = lib().slokv_paged_decode_workspace_bytes(index, num_q_heads, num_kv_heads, HEAD_DIM)
+        if n == 0:
+            raise SlokvError(f"unsupported decode geometry Hq={num_q_heads} Hkv={num_kv_heads}")
+        _workspace_bytes[key] = n
+    return n
 
 
 def flash_attn_with_kvcache_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -75,44 +97,49 @@ def flash_attn_with_kvcache_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     """
     four = is_int4_cache(k_cache)
     if four:
-        NB, bs, Hkv = int4_geometry(k_cache, v_cache)
+        pool = int4_geometry(k_cache, v_cache)
     else:
-        NB, bs, Hkv = _dense_geometry(k_cache, v_cache, (torch.bfloat16, torch.float16))
+        pool = _dense_geometry(k_cache, v_cache, _DECODE_DTYPES)
         if q.dtype != k_cache.dtype:
             raise SlokvError("q and cache dtypes differ")
+    NB, bs, Hkv, k_block, v_block = pool
     dev = require_cuda(q, k_cache, v_cache, scores, cache_seqlens, block_table, score_rows, out)
-    B, Hq, out = check_decode_args(q, cache_seqlens, block_table, out, HEAD_DIM)
-    _check_scores(scores, score_rows, B, Hkv)
+    B, Hq, out = check_decode_args(q, cache_seqlens, block_table, out)
+    rows, width, row, head, rows_ptr = _check_scores(scores, score_rows, B, Hkv)
     if Hq % Hkv:
         raise SlokvError("query heads must divide by the KV heads")
     if B == 0:
         return out
-    width = scores.shape[2] if max_seqlen_k is None else min(int(max_seqlen_k), scores.shape[2])
+    if max_seqlen_k is not None:
+        width = min(int(max_seqlen_k), width)
     if width <= 0:
         raise SlokvError("scores have no columns (or max_seqlen_k is not positive)")
-    scale = float(softmax_scale) if softmax_scale is not None else HEAD_DIM ** -0.5
-    with torch.cuda.device(dev):
-        stride = (width + 3) // 4 * 4
-        logits = torch.empty(B, Hq, stride, dtype=torch.float32, device=dev)
-        lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
-        err, stream = buffers.error_word(dev).data_ptr(), stream_ptr(dev)
+    scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
+    stride = (width + 3) // 4 * 4
+    with on_device(dev) as stream:
+        nbytes = (decode_int4_workspace_bytes if four else _decode_workspace_bytes)(dev.index, Hq,
+                                                                                    Hkv)
+        # one scratch: the decode's workspace, the scores of this step, their denominators
+        logits_at = (nbytes + 255) // 256 * 256
+        lse_at = logits_at + 4 * B * Hq * stride
+        scratch = torch.empty(lse_at + 4 * B * Hq, dtype=torch.uint8, device=dev)
+        ws = scratch.data_ptr()
+        logits, lse, err = ws + logits_at, ws + lse_at, buffers.error_word(dev).data_ptr()
         if four:
-            _decode_int4(q, k_cache, v_cache, cache_seqlens, block_table, scale, out, logits, lse)
+            launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens, block_table, scale, B, Hq,
+                               out, ws, nbytes, err, stream, logits, stride, lse)
         else:
-            nbytes = lib().slokv_paged_decode_workspace_bytes(-1, Hq, Hkv, HEAD_DIM)
-            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+            qs, os = q.stride(), out.stride()
             check(lib().slokv_paged_decode_logits(
-                out.data_ptr(), out.stride(0), out.stride(2), q.data_ptr(), q.stride(0),
-                q.stride(2), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
-                v_cache.stride(0), NB, bs, Hq, Hkv, HEAD_DIM, block_table.data_ptr(),
-                block_table.stride(0), block_table.shape[1], cache_seqlens.data_ptr(), B, scale,
-                _lib.dtype_code(q.dtype), logits.data_ptr(), stride, lse.data_ptr(),
-                ws.data_ptr(), nbytes, err, stream), "paged_decode_logits")
+                out.data_ptr(), os[0], os[2], q.data_ptr(), qs[0], qs[2], k_cache.data_ptr(),
+                v_cache.data_ptr(), k_block, v_block, NB, bs, Hq, Hkv, HEAD_DIM,
+                block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                cache_seqlens.data_ptr(), B, scale, _DECODE_DTYPES[q.dtype], logits, stride, lse, ws,
+                nbytes, err, stream), "paged_decode_logits")
         check(lib().slokv_kv_scores_accumulate(
-            scores.data_ptr(), scores.stride(0), scores.stride(1), width, scores.shape[0],
-            None if score_rows is None else score_rows.data_ptr(), logits.data_ptr(), stride,
-            lse.data_ptr(), cache_seqlens.data_ptr(), B, Hq, Hkv, block_table.shape[1] * bs,
-            float(decay), err, stream), "kv_scores_accumulate")
+            scores.data_ptr(), row, head, width, rows, rows_ptr, logits, stride, lse,
+            cache_seqlens.data_ptr(), B, Hq, Hkv, block_table.shape[1] * bs, float(decay), err,
+            stream), "kv_scores_accumulate")
     return out
 
 
@@ -135,33 +162,29 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     if keep < 1 or recent < 0 or recent > keep:
         raise SlokvError("kv_evict needs keep >= 1 and 0 <= recent <= keep")
     if is_int4_cache(k_cache):
-        NB, bs, Hkv = int4_geometry(k_cache, v_cache)
-        dtype, strides = _lib.DTYPE_INT4, (_block_stride(k_cache), _block_stride(v_cache))
+        NB, bs, Hkv, k_block, v_block = int4_geometry(k_cache, v_cache)
+        dtype = _lib.DTYPE_INT4
     else:
-        NB, bs, Hkv = _dense_geometry(k_cache, v_cache,
-                                      (torch.bfloat16, torch.float16, torch.float32))
-        es = k_cache.element_size()
-        dtype = _lib.dtype_code(k_cache.dtype)
-        strides = (k_cache.stride(0) * es, v_cache.stride(0) * es)
+        NB, bs, Hkv, k_block, v_block = _dense_geometry(k_cache, v_cache, _EVICT_DTYPES)
+        dtype, es = _EVICT_DTYPES[k_cache.dtype], k_cache.element_size()
+        k_block, v_block = k_block * es, v_block * es
     dev = require_cuda(k_cache, v_cache, scores, cache_seqlens, block_table, score_rows)
     _i32_contig("cache_seqlens", cache_seqlens)
     B = cache_seqlens.numel()
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(-1) != 1 \
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1 \
             or block_table.shape[0] < B or block_table.shape[1] == 0:
         raise SlokvError("block_table must be int32 [batch, pages] with a contiguous last dim")
-    _check_scores(scores, score_rows, B, Hkv)
+    rows, width, row, head, rows_ptr = _check_scores(scores, score_rows, B, Hkv)
     new_lens = torch.empty(B, dtype=torch.int32, device=dev)
     index = torch.empty(B, Hkv, keep, dtype=torch.int32, device=dev) if return_index else None
     if B:
-        with torch.cuda.device(dev):
-            nbytes = lib().slokv_kv_evict_workspace_bytes(B, Hkv, keep, scores.shape[2])
+        with on_device(dev) as stream:
+            nbytes = lib().slokv_kv_evict_workspace_bytes(B, Hkv, keep, width)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             check(lib().slokv_kv_evict(
-                k_cache.data_ptr(), v_cache.data_ptr(), *strides, NB, bs, Hkv, HEAD_DIM, dtype,
-                block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-                cache_seqlens.data_ptr(), B, scores.data_ptr(), scores.stride(0),
-                scores.stride(1), scores.shape[2], scores.shape[0],
-                None if score_rows is None else score_rows.data_ptr(), keep, recent,
-                new_lens.data_ptr(), None if index is None else index.data_ptr(), ws.data_ptr(),
-                nbytes, buffers.error_word(dev).data_ptr(), stream_ptr(dev)), "kv_evict")
+                k_cache.data_ptr(), v_cache.data_ptr(), k_block, v_block, NB, bs, Hkv, HEAD_DIM,
+                dtype, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                cache_seqlens.data_ptr(), B, scores.data_ptr(), row, head, width, rows, rows_ptr,
+                keep, recent, new_lens.data_ptr(), None if index is None else index.data_ptr(),
+                ws.data_ptr(), nbytes, buffers.error_word(dev).data_ptr(), stream), "kv_evict")
     return (new_lens, index) if return_index else new_lens

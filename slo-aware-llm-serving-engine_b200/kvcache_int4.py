@@ -18,13 +18,16 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import SlokvError, buffers, check, lib, require_cuda, stream_ptr
+from ._lib import SlokvError, buffers, check, lib, on_device, require_cuda
 from .kvcache import _i32_contig, _varlen_attention
 
 HEAD_DIM = 128
 TILE_TOKENS = 64
 ROW_BYTES = 72          # 64 bytes of codes, 2 x (scale, minimum) in bf16
 _WIDE_PAGE = 128        # tokens of a page that rows are widened to for prefill
+
+_Q_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_STORE_DTYPES = {**_Q_DTYPES, torch.float32: _lib.DTYPE_F32}
 
 
 def is_int4_cache(cache: torch.Tensor) -> bool:
@@ -40,25 +43,28 @@ def int4_pool_shape(num_blocks: int, block_size: int, num_kv_heads: int):
 
 
 def int4_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor):
-    """(num_blocks, block_size, num_kv_heads) of a 4-bit pool, checked."""
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if not is_int4_cache(c):
-            raise SlokvError(f"{name} must be a uint8 4-bit pool [num_blocks, num_kv_heads, "
-                             f"block_size * {ROW_BYTES}]")
-        if c.shape[2] == 0 or c.shape[2] % (TILE_TOKENS * ROW_BYTES):
-            raise SlokvError(f"{name}: the last dim must be block_size * {ROW_BYTES} bytes, "
-                             f"block_size a multiple of {TILE_TOKENS}")
-        if c.stride(2) != 1 or (c.shape[1] > 1 and c.stride(1) != c.shape[2]):
-            raise SlokvError(f"{name} blocks must be contiguous")
-        if c.shape[0] > 1 and c.stride(0) < c.shape[1] * c.shape[2]:
-            raise SlokvError(f"{name} blocks must not overlap")
-    if v_cache.shape != k_cache.shape:
+    """(num_blocks, block_size, num_kv_heads, K and V block strides in bytes) of a 4-bit
+    pool, checked."""
+    if k_cache.shape != v_cache.shape:
         raise SlokvError("k_cache and v_cache shapes differ")
-    return k_cache.shape[0], k_cache.shape[2] // ROW_BYTES, k_cache.shape[1]
-
-
-def _block_stride(c: torch.Tensor) -> int:
-    return c.stride(0) if c.shape[0] > 1 else c.shape[1] * c.shape[2]
+    strides = []
+    for c in (k_cache, v_cache):
+        if not is_int4_cache(c):
+            raise SlokvError("k_cache / v_cache must be uint8 4-bit pools [num_blocks, "
+                             f"num_kv_heads, block_size * {ROW_BYTES}]")
+        nb, h, size = c.shape
+        if size == 0 or size % (TILE_TOKENS * ROW_BYTES):
+            raise SlokvError(f"a 4-bit pool's last dim must be block_size * {ROW_BYTES} bytes, "
+                             f"block_size a multiple of {TILE_TOKENS}")
+        block, head, one = c.stride()
+        if one != 1 or (h > 1 and head != size):
+            raise SlokvError("a 4-bit pool's blocks must be contiguous")
+        if nb <= 1:
+            block = h * size
+        elif block < h * size:
+            raise SlokvError("a 4-bit pool's blocks must not overlap")
+        strides.append(block)
+    return nb, size // ROW_BYTES, h, strides[0], strides[1]
 
 
 def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -74,11 +80,14 @@ def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
     N, H, D = key.shape
     if D != HEAD_DIM:
         raise SlokvError(f"the 4-bit pool has head_dim {HEAD_DIM}, not {D}")
-    if key.dtype != value.dtype or key.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    dtype = key.dtype
+    if value.dtype != dtype or dtype not in _STORE_DTYPES:
         raise SlokvError("key and value must both be bf16, f16 or fp32")
-    if key.stride(-1) != 1 or value.stride(-1) != 1:
+    k_row, k_head, k_one = key.stride()
+    v_row, v_head, v_one = value.stride()
+    if k_one != 1 or v_one != 1:
         raise SlokvError("key and value need a contiguous last dimension")
-    NB, bs, Hkv = int4_geometry(k_cache, v_cache)
+    NB, bs, Hkv, k_block, v_block = int4_geometry(k_cache, v_cache)
     if Hkv != H:
         raise SlokvError(f"the pool has {Hkv} KV heads, key / value {H}")
     dev = require_cuda(key, value, k_cache, v_cache, slot_mapping)
@@ -87,76 +96,81 @@ def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
         raise SlokvError("slot_mapping must have one entry per token")
     if N == 0:
         return
-    with torch.cuda.device(dev):
+    with on_device(dev) as stream:
         check(lib().slokv_kv_append_int4(
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-            value.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), _block_stride(k_cache),
-            _block_stride(v_cache), slot_mapping.data_ptr(), N, H, D, bs, NB,
-            _lib.dtype_code(key.dtype), buffers.error_word(dev).data_ptr(), stream_ptr(dev)),
-            "kv_append_int4")
+            key.data_ptr(), k_row, k_head, value.data_ptr(), v_row, v_head, k_cache.data_ptr(),
+            v_cache.data_ptr(), k_block, v_block, slot_mapping.data_ptr(), N, H, D, bs, NB,
+            _STORE_DTYPES[dtype], buffers.error_word(dev).data_ptr(), stream), "kv_append_int4")
 
 
 def int4_decode(cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
     """fp32 values [N, Hkv, 128] of the rows at `slots` ([N] int32) of one side of a
     4-bit pool (e4m3_decode's counterpart); slot -1 gives zeros."""
-    NB, bs, H = int4_geometry(cache, cache)
+    NB, bs, H, block, _ = int4_geometry(cache, cache)
     dev = require_cuda(cache, slots)
     _i32_contig("slots", slots)
-    out = torch.empty(slots.numel(), H, HEAD_DIM, dtype=torch.float32, device=dev)
-    if slots.numel():
-        with torch.cuda.device(dev):
+    n = slots.numel()
+    out = torch.empty(n, H, HEAD_DIM, dtype=torch.float32, device=dev)
+    if n:
+        with on_device(dev) as stream:
             check(lib().slokv_int4_decode(
-                cache.data_ptr(), _block_stride(cache), slots.data_ptr(), slots.numel(), H,
-                HEAD_DIM, bs, NB, out.data_ptr(), buffers.error_word(dev).data_ptr(),
-                stream_ptr(dev)), "int4_decode")
+                cache.data_ptr(), block, slots.data_ptr(), n, H, HEAD_DIM, bs, NB, out.data_ptr(),
+                buffers.error_word(dev).data_ptr(), stream), "int4_decode")
     return out
 
 
-def check_decode_args(q, cache_seqlens, block_table, out, head_dim):
+def check_decode_args(q, cache_seqlens, block_table, out):
     """Argument checks that the paged decodes of this package's 4-bit and scored
     paths share; returns (batch, query heads, out)."""
-    if q.dim() != 4 or q.shape[1] != 1 or q.shape[3] != head_dim:
-        raise SlokvError(f"paged decode expects q of shape [batch, 1, heads, {head_dim}]")
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.stride(-1) != 1:
+    if q.dim() != 4:
+        raise SlokvError(f"paged decode expects q of shape [batch, 1, heads, {HEAD_DIM}]")
+    B, one, Hq, D = q.shape
+    if one != 1 or D != HEAD_DIM:
+        raise SlokvError(f"paged decode expects q of shape [batch, 1, heads, {HEAD_DIM}]")
+    if q.dtype not in _Q_DTYPES or q.stride(3) != 1:
         raise SlokvError("q must be bf16 or f16 with a contiguous last dimension")
-    B, _, Hq, _ = q.shape
     _i32_contig("cache_seqlens", cache_seqlens)
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(-1) != 1:
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
         raise SlokvError("block_table must be int32 [batch, pages] with a contiguous last dim")
-    if block_table.shape[0] < B or cache_seqlens.numel() < B:
+    rows, width = block_table.shape
+    if rows < B or cache_seqlens.numel() < B:
         raise SlokvError("block_table / cache_seqlens have fewer rows than q")
-    if block_table.shape[1] == 0:
+    if width == 0:
         raise SlokvError("block_table has no columns")
     if out is None:
-        out = torch.empty(B, 1, Hq, head_dim, dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.stride(-1) != 1 or not out.is_cuda:
-        raise SlokvError("out must match q's shape, dtype and device with a contiguous last dim")
+        out = torch.empty(B, 1, Hq, HEAD_DIM, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.stride(3) != 1:
+        raise SlokvError("out must match q's shape and dtype with a contiguous last dim")
     return B, Hq, out
 
 
-def _decode_int4(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out,
-                 logits=None, lse=None):
-    NB, bs, Hkv = int4_geometry(k_cache, v_cache)
-    dev = require_cuda(q, k_cache, v_cache, cache_seqlens, block_table, out)
-    B, Hq, out = check_decode_args(q, cache_seqlens, block_table, out, HEAD_DIM)
-    if B == 0:
-        return out
-    scale = float(softmax_scale) if softmax_scale is not None else HEAD_DIM ** -0.5
-    with torch.cuda.device(dev):
-        nbytes = lib().slokv_paged_decode_int4_workspace_bytes(-1, Hq, Hkv, HEAD_DIM)
-        if nbytes == 0:
-            raise SlokvError(f"unsupported 4-bit decode geometry Hq={Hq} Hkv={Hkv}")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(lib().slokv_paged_decode_int4(
-            out.data_ptr(), out.stride(0), out.stride(2), q.data_ptr(), q.stride(0), q.stride(2),
-            k_cache.data_ptr(), v_cache.data_ptr(), _block_stride(k_cache),
-            _block_stride(v_cache), NB, bs, Hq, Hkv, HEAD_DIM, block_table.data_ptr(),
-            block_table.stride(0), block_table.shape[1], cache_seqlens.data_ptr(), B, scale,
-            _lib.dtype_code(q.dtype), None if logits is None else logits.data_ptr(),
-            0 if logits is None else logits.stride(1), None if lse is None else lse.data_ptr(),
-            ws.data_ptr(), nbytes, buffers.error_word(dev).data_ptr(), stream_ptr(dev)),
-            "paged_decode_int4")
-    return out
+_workspace_bytes = {}   # (device, Hq, Hkv) -> bytes: a property of the device
+
+
+def decode_int4_workspace_bytes(index: int, num_q_heads: int, num_kv_heads: int) -> int:
+    key = (index, num_q_heads, num_kv_heads)
+    n = _workspace_bytes.get(key)
+    if n is None:
+        n = lib().slokv_paged_decode_int4_workspace_bytes(index, num_q_heads, num_kv_heads,
+                                                          HEAD_DIM)
+        if n == 0:
+            raise SlokvError(f"unsupported 4-bit decode geometry Hq={num_q_heads} "
+                             f"Hkv={num_kv_heads}")
+        _workspace_bytes[key] = n
+    return n
+
+
+def launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens, block_table, scale, B, Hq, out,
+                       workspace, nbytes, err, stream, logits=None, logits_stride=0, lse=None):
+    """slokv_paged_decode_int4 on checked arguments; workspace, logits and lse are addresses."""
+    NB, bs, Hkv, k_block, v_block = pool
+    qs, os = q.stride(), out.stride()
+    check(lib().slokv_paged_decode_int4(
+        out.data_ptr(), os[0], os[2], q.data_ptr(), qs[0], qs[2], k_cache.data_ptr(),
+        v_cache.data_ptr(), k_block, v_block, NB, bs, Hq, Hkv, HEAD_DIM, block_table.data_ptr(),
+        block_table.stride(0), block_table.shape[1], cache_seqlens.data_ptr(), B, scale,
+        _Q_DTYPES[q.dtype], logits, logits_stride, lse, workspace, nbytes, err, stream),
+        "paged_decode_int4")
 
 
 def flash_attn_with_kvcache_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -169,7 +183,18 @@ def flash_attn_with_kvcache_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache
     aligned with even strides; cache_seqlens: [B] int32 including the token stored this
     step (0: the row's output is zero); block_table: [B, W] int32.
     """
-    return _decode_int4(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out)
+    pool = int4_geometry(k_cache, v_cache)
+    dev = require_cuda(q, k_cache, v_cache, cache_seqlens, block_table, out)
+    B, Hq, out = check_decode_args(q, cache_seqlens, block_table, out)
+    if B == 0:
+        return out
+    scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
+    with on_device(dev) as stream:
+        nbytes = decode_int4_workspace_bytes(dev.index, Hq, pool[2])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens, block_table, scale, B, Hq, out,
+                           ws.data_ptr(), nbytes, buffers.error_word(dev).data_ptr(), stream)
+    return out
 
 
 def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
@@ -191,7 +216,7 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
             or q.stride(-1) != 1:
         raise SlokvError(f"q must be bf16/f16 [tokens, heads, {HEAD_DIM}] with a contiguous last "
                          "dim")
-    NB, bs, Hkv = int4_geometry(k_cache, v_cache)
+    NB, bs, Hkv, k_block, v_block = int4_geometry(k_cache, v_cache)
     dev = require_cuda(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, out)
     _i32_contig("cu_seqlens_q", cu_seqlens_q)
     _i32_contig("cu_seqlens_k", cu_seqlens_k)
@@ -210,14 +235,14 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
     if q.shape[0] == 0 or rows <= 0 or int(max_seqlen_q) <= 0:
         return out
     pages = max(1, (int(max_seqlen_k) + _WIDE_PAGE - 1) // _WIDE_PAGE)
-    with torch.cuda.device(dev):
+    with on_device(dev) as stream:
         wide = torch.empty(2, rows * pages, _WIDE_PAGE, Hkv, HEAD_DIM, dtype=q.dtype, device=dev)
         table = torch.empty(rows, pages, dtype=torch.int32, device=dev)
         check(lib().slokv_int4_rows_widen(
-            k_cache.data_ptr(), v_cache.data_ptr(), _block_stride(k_cache),
-            _block_stride(v_cache), NB, bs, Hkv, HEAD_DIM, block_table.data_ptr(),
-            block_table.stride(0), block_table.shape[1], cu_seqlens_k.data_ptr(), rows, pages,
-            wide[0].data_ptr(), wide[1].data_ptr(), table.data_ptr(), _lib.dtype_code(q.dtype),
-            buffers.error_word(dev).data_ptr(), stream_ptr(dev)), "int4_rows_widen")
+            k_cache.data_ptr(), v_cache.data_ptr(), k_block, v_block, NB, bs, Hkv, HEAD_DIM,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+            cu_seqlens_k.data_ptr(), rows, pages, wide[0].data_ptr(), wide[1].data_ptr(),
+            table.data_ptr(), _Q_DTYPES[q.dtype], buffers.error_word(dev).data_ptr(), stream),
+            "int4_rows_widen")
         return _varlen_attention(q, wide[0], wide[1], cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
                                  softmax_scale, causal, table, out, None)

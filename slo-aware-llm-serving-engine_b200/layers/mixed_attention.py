@@ -7,7 +7,8 @@ for the rest (paged through `prefill_tables` when any row has history, else on
 the contiguous k/v of the chunk).  Both kernels write straight into one [T, Hq,
 D] output, so no concatenation copy is made.  `forward_mixed_fp8` is the same
 step over an FP8-E4M3 pool: quantising store, FP8 decode, and prefill rows with
-history attended through pages dequantised for the step.
+history attended through pages dequantised for the step.  A 4-bit pool takes
+`forward_mixed` with its own store, decode and varlen functions.
 """
 from dataclasses import dataclass
 
@@ -31,7 +32,10 @@ class MixedAttentionContext:
     prefill_has_history: bool = True
 
 
-def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn):
+def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn, *,
+                  decode_fn=flash_attn_with_kvcache, varlen_fn=flash_attn_varlen_func):
+    """store_fn stores all rows, decode_fn attends the decode rows and varlen_fn the prefill
+    rows that have history; a 4-bit pool passes its own three, a scored layer its decode_fn."""
     meta = context.mixed
     if not k_cache.numel() or not v_cache.numel():
         raise RuntimeError("mixed forward requires an allocated BF16 KV pool")
@@ -40,18 +44,16 @@ def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn):
     n = d + meta.num_prefill_tokens
     out = torch.empty((n,) + tuple(q.shape[1:]), dtype=q.dtype, device=q.device)
     if d:
-        flash_attn_with_kvcache(q[:d].unsqueeze(1), k_cache, v_cache,
-                                cache_seqlens=meta.decode_lens, block_table=meta.decode_tables,
-                                softmax_scale=scale, causal=True, out=out[:d].unsqueeze(1))
+        decode_fn(q[:d].unsqueeze(1), k_cache, v_cache,
+                  cache_seqlens=meta.decode_lens, block_table=meta.decode_tables,
+                  softmax_scale=scale, causal=True, out=out[:d].unsqueeze(1))
     if meta.num_prefill_tokens:
         history = meta.prefill_has_history
-        flash_attn_varlen_func(q[d:n], k_cache if history else k[d:n],
-                               v_cache if history else v[d:n],
-                               cu_seqlens_q=meta.prefill_cu_q, cu_seqlens_k=meta.prefill_cu_k,
-                               max_seqlen_q=meta.max_q, max_seqlen_k=meta.max_k,
-                               softmax_scale=scale, causal=True,
-                               block_table=meta.prefill_tables if history else None,
-                               out=out[d:n])
+        attend = varlen_fn if history else flash_attn_varlen_func
+        attend(q[d:n], k_cache if history else k[d:n], v_cache if history else v[d:n],
+               cu_seqlens_q=meta.prefill_cu_q, cu_seqlens_k=meta.prefill_cu_k,
+               max_seqlen_q=meta.max_q, max_seqlen_k=meta.max_k, softmax_scale=scale,
+               causal=True, block_table=meta.prefill_tables if history else None, out=out[d:n])
     return out
 
 

@@ -11,7 +11,8 @@ kv_cache[0, l] / kv_cache[1, l].
 
 FP8-E4M3 pools keep uint8 codes in the same layout plus fp32 scales
 k_scale/v_scale [num_layers, num_blocks, Hkv_local]; block_bytes counts the
-scales.  A reused page never inherits an old amax without any call from the
+scales.  4-bit pools are one uint8 tensor [2, num_layers, num_blocks, Hkv_local,
+block_size * 72] whose pages carry their own scales.  A reused page never inherits an old amax without any call from the
 block manager: the quantising append ignores a block's stored scale when its
 write starts at offset 0, where every newly assigned block is first written
 (reset_blocks remains as an eager helper for tools that want clean scales).
@@ -20,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from . import kvcache
+from . import kvcache, kvcache_int4
 
 
 def tp_shard(num_heads: int, num_kv_heads: int, tp_size: int, rank: int):
@@ -39,6 +40,8 @@ def block_bytes(num_layers: int, block_size: int, num_kv_heads: int, head_dim: i
     """Bytes one block id occupies over all layers, K and V (plus FP8 scales)."""
     if kv_dtype == "fp8":
         return 2 * num_layers * (block_size * num_kv_heads * head_dim + num_kv_heads * 4)
+    if kv_dtype == "int4":
+        return 2 * num_layers * block_size * num_kv_heads * kvcache_int4.ROW_BYTES
     if kv_dtype in ("bf16", "f16"):
         return 2 * num_layers * block_size * num_kv_heads * head_dim * 2
     raise ValueError(f"unknown kv dtype {kv_dtype}")
@@ -77,6 +80,12 @@ class KVPool:
             self.k_scale = torch.zeros(num_layers, num_blocks, num_kv_heads, dtype=torch.float32,
                                        device=device)
             self.v_scale = torch.zeros_like(self.k_scale)
+        elif kv_dtype == "int4":
+            if head_dim != kvcache_int4.HEAD_DIM:
+                raise ValueError(f"4-bit pools have head_dim {kvcache_int4.HEAD_DIM}")
+            page = kvcache_int4.int4_pool_shape(num_blocks, block_size, num_kv_heads)
+            self.kv_cache = torch.zeros((2, num_layers) + page, dtype=torch.uint8, device=device)
+            self.k_scale = self.v_scale = None
         else:
             dt = torch.bfloat16 if kv_dtype == "bf16" else torch.float16
             self.kv_cache = torch.empty(shape, dtype=dt, device=device)

@@ -26,7 +26,9 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
+from .eviction import kv_evict
 from .kvcache import qk_norm_rope_append
+from .kvcache_int4 import is_int4_cache
 from .layers.attention import Attention
 from .layers.linear import RowParallelAllReduce
 from .pool import KVPool, tp_shard
@@ -166,7 +168,8 @@ class Qwen3Model:
                 x, res = add_rms_norm(h, res, lw.ln1, eps)
             qkv = F.linear(x, lw.wqkv)
             if (self.fused_qk_norm_rope and type(lw.attn) is Attention
-                    and lw.attn.k_scale is None and lw.attn.k_cache.numel()):
+                    and lw.attn.k_scale is None and lw.attn.k_cache.numel()
+                    and not is_int4_cache(lw.attn.k_cache)):
                 ctx = get_context()
                 cold = ctx.is_prefill and ctx.block_tables is None   # attends on its own rows
                 out = qk_norm_rope_append(qkv, self.hq, self.hkv, lw.qn, lw.kn, eps, positions,
@@ -202,10 +205,15 @@ class GreedyRunner:
     (cold prompts: varlen on the step's own k/v, as `prepare_prefill` sets it
     up without a prefix cache); decode builds slot_mapping / context_lens /
     block_tables like `prepare_decode` and can be captured in a CUDA graph.
+
+    kv_dtype: "bf16", "fp8" or "int4".  With `score` every layer accumulates the decode
+    steps' attention weights, and `evict(keep, recent)` cuts all sequences in place; the
+    next tokens then keep their positions in the text and take the freed slots.
     """
 
     def __init__(self, model: Qwen3Model, prompt_lens, max_new: int, block_size: int = 256,
-                 seed: int = 0, spare_blocks: int = 0, kv_dtype: str = "bf16"):
+                 seed: int = 0, spare_blocks: int = 0, kv_dtype: str = "bf16",
+                 score: bool = False):
         self.model, self.bs = model, block_size
         self.lens = [int(n) for n in prompt_lens]
         self.B = len(self.lens)
@@ -224,6 +232,12 @@ class GreedyRunner:
             cur += n
         self.tables = torch.tensor(tables, dtype=torch.int32, device=dev)
         self.graph = None
+        self.scores = None
+        if score:
+            self.scores = torch.zeros(model.cfg.num_layers, self.B, model.hkv,
+                                      self.W * block_size, dtype=torch.float32, device=dev)
+        for i, attn in enumerate(model.attention_modules()):
+            attn.scores = None if self.scores is None else self.scores[i]
 
     def _slots(self, b: int, start: int, stop: int) -> list[int]:
         row = self.tables[b].tolist()
@@ -257,13 +271,16 @@ class GreedyRunner:
             out[b:e] = self.model.logits(h[cu_t[1:].long() - 1]).argmax(dim=-1)
             b = e
         self.pos = torch.tensor(self.lens, dtype=torch.int64, device=dev)
+        self.cached = self.pos.clone()       # tokens in the cache: fewer than pos after evict()
+        if self.scores is not None:
+            self.scores.zero_()
         return out
 
-    def _decode_body(self, ids, pos, ctx_lens, slots):
+    def _decode_body(self, ids, pos, cached, ctx_lens, slots):
         """One decode forward over static buffers (graph-capturable)."""
-        blk = torch.gather(self.tables, 1, (pos // self.bs).unsqueeze(1)).squeeze(1)
-        slots.copy_(blk * self.bs + (pos % self.bs).to(torch.int32))
-        ctx_lens.copy_((pos + 1).to(torch.int32))
+        blk = torch.gather(self.tables, 1, (cached // self.bs).unsqueeze(1)).squeeze(1)
+        slots.copy_(blk * self.bs + (cached % self.bs).to(torch.int32))
+        ctx_lens.copy_((cached + 1).to(torch.int32))
         set_context(False, None, None, 0, 0, slots, ctx_lens, self.tables)
         h = self.model.forward(ids, pos)
         reset_context()
@@ -279,24 +296,45 @@ class GreedyRunner:
             self._pos = torch.zeros(self.B, dtype=torch.int64, device=dev)
             self._lens = torch.zeros(self.B, dtype=torch.int32, device=dev)
             self._slots_buf = torch.zeros(self.B, dtype=torch.int32, device=dev)
+            self._cached = torch.zeros(self.B, dtype=torch.int64, device=dev)
             self._ids.copy_(tokens)
             self._pos.copy_(self.pos)
-            self._decode_body(self._ids, self._pos, self._lens, self._slots_buf)  # warm-up
+            self._cached.copy_(self.cached)
+            before = None if self.scores is None else self.scores.clone()
+            self._decode_body(self._ids, self._pos, self._cached, self._lens,
+                              self._slots_buf)  # warm-up
+            if before is not None:               # the replay below scores this step again
+                self.scores.copy_(before)
             torch.cuda.synchronize(dev)
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
-                self._next = self._decode_body(self._ids, self._pos, self._lens, self._slots_buf)
+                self._next = self._decode_body(self._ids, self._pos, self._cached, self._lens,
+                                               self._slots_buf)
         if use_graph:
             self._ids.copy_(tokens)
             self._pos.copy_(self.pos)
+            self._cached.copy_(self.cached)
             self.graph.replay()
             nxt = self._next.clone()
         else:
             lens = torch.empty(self.B, dtype=torch.int32, device=dev)
             slots = torch.empty(self.B, dtype=torch.int32, device=dev)
-            nxt = self._decode_body(tokens, self.pos, lens, slots)
+            nxt = self._decode_body(tokens, self.pos, self.cached, lens, slots)
         self.pos += 1
+        self.cached += 1
         return nxt
+
+    @torch.inference_mode()
+    def evict(self, keep: int, recent: int) -> torch.Tensor:
+        """Cut every sequence longer than `keep` tokens to its `recent` last and its
+        heaviest, per layer and KV head; returns the cache lengths [B]."""
+        if self.scores is None:
+            raise RuntimeError("evict() needs a runner made with score=True")
+        lens = self.cached.to(torch.int32)
+        for attn in self.model.attention_modules():
+            new = kv_evict(attn.k_cache, attn.v_cache, attn.scores, lens, self.tables, keep, recent)
+        self.cached.copy_(new)
+        return new
 
     def release(self):
         """Drop the captured graph (it holds NCCL calls under TP)."""

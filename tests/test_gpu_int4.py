@@ -3,8 +3,9 @@ restatements (tests/int4_reference.py).
 
 Tolerances.  Stored bytes are compared exactly.  Decode (derived from the kernel's
 arithmetic, u = 2^-24, half a step of fp32):
-  * the rounding of p s to f16 meets (c - 8) s: 2^-11 sum_t w_t s_t |c_t - 8| (plus
-    nothing below 2^-29 of the largest scale, which the cases do not reach);
+  * the rounding of p s to f16 meets c s (bf16 outputs) or (c - 8) s (f16 outputs):
+    2^-11 sum_t w_t s_t c_t, or |c_t - 8| (plus nothing below 2^-29 of the largest scale,
+    which the cases do not reach);
   * an error e in a score changes its weight by a factor within 1 +- 2 e: e <= (128 + 16)
     products and sums in fp32, each within u of their absolute sum, so e <= 400 u
     scale sum_d |q_d| (15 s + |m|) with the tensor core's truncation counted double;
@@ -61,7 +62,8 @@ def decode_bound(q, k, v, ks, vs, kmin_abs, w, out, scale, dtype):
     rep = lambda x: x.repeat_interleave(G, 1)
     s_dim = rep(vs).repeat_interleave(64, -1)                       # [n, Hq, 128]
     vv = rep(v)
-    centre = (vv - (rep(kmin_abs[1]).repeat_interleave(64, -1) + 8 * s_dim)).abs()
+    middle = 8 if dtype == torch.float16 else 0
+    centre = (vv - (rep(kmin_abs[1]).repeat_interleave(64, -1) + middle * s_dim)).abs()
     k_abs = rep(kmin_abs[0].abs() + 15 * ks).repeat_interleave(64, -1)
     e = 400 * U * abs(scale) * torch.einsum("hd,nhd->hn", q.double().abs(), k_abs).max(-1).values
     wv = torch.einsum("hn,nhd->hd", w, vv.abs())
