@@ -124,16 +124,20 @@ SIGNATURES = {
     "slokv_paged_decode_int4_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32]),
     "slokv_paged_decode_int4": (ctypes.c_int, [
         _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64,
-        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp, _c_i64, _c_i32, _c_vp, _c_i32,
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_vp, _c_i64, _c_i32, _c_vp, _c_vp, _c_i32,    # tables, stride, width, rows, lens, batch
         _c_f32, _c_i32, _c_vp, _c_i64, _c_vp,           # scale, dtype, logits, stride, lse
         _c_vp, _c_sz, _c_vp, _c_vp]),
+    "slokv_int4_rows_expand": (ctypes.c_int, [
+        _c_vp, _c_vp, _c_i32, _c_i32, _c_vp, _c_vp, _c_vp]),
     "slokv_paged_decode_logits": (ctypes.c_int, [
         _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64,
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp, _c_i64, _c_i32, _c_vp, _c_i32,
         _c_f32, _c_i32, _c_vp, _c_i64, _c_vp, _c_vp, _c_sz, _c_vp, _c_vp]),
     "slokv_kv_scores_accumulate": (ctypes.c_int, [
         _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_vp,   # scores, strides, width, rows, map
-        _c_vp, _c_i64, _c_vp, _c_vp, _c_i32, _c_i32, _c_i32,   # logits, lse, lens, B, Hq, Hkv
+        _c_vp, _c_i64, _c_i32, _c_vp, _c_vp,            # logits, stride, pairs, lse, lens
+        _c_i32, _c_i32, _c_i32,                         # B, Hq, Hkv
         _c_i64, _c_f32, _c_vp, _c_vp]),                 # max context, decay, err, stream
     "slokv_kv_evict_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32]),
     "slokv_kv_evict": (ctypes.c_int, [

@@ -254,6 +254,28 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// The queries of a short prefill as decode rows: query token i of row r attends to the
+// first k_len - q_len + i + 1 cached tokens of table row r.  Tokens that no row names get
+// the length -1.
+__global__ void int4_rows_expand_kernel(const int32_t *__restrict__ cu_q,
+                                        const int32_t *__restrict__ cu_k, int32_t rows,
+                                        int32_t tokens, int32_t *__restrict__ table_rows,
+                                        int32_t *__restrict__ lens) {
+  const int32_t t = blockIdx.x * blockDim.x + threadIdx.x;
+  if (t >= tokens) return;
+  // the last row that starts at or before t
+  int32_t lo = 0, hi = rows - 1;
+  while (lo < hi) {
+    const int32_t mid = (lo + hi + 1) >> 1;
+    if (__ldg(cu_q + mid) <= t) lo = mid; else hi = mid - 1;
+  }
+  const int32_t first = __ldg(cu_q + lo), last = __ldg(cu_q + lo + 1);
+  const bool named = t >= first && t < last;
+  const int32_t keys = __ldg(cu_k + lo + 1) - __ldg(cu_k + lo);
+  table_rows[t] = lo;
+  lens[t] = named ? max(0, keys - (last - t) + 1) : -1;
+}
+
 bool pool_ok(const void *base, int64_t block_stride, int32_t hkv, int32_t block_size) {
   return !(reinterpret_cast<uintptr_t>(base) & 15u) && !(block_stride & 15) &&
          block_stride >= static_cast<int64_t>(hkv) * block_size * kRowBytes;
@@ -374,4 +396,17 @@ extern "C" int slokv_int4_rows_widen(const void *k_cache, const void *v_cache,
   };
   return dst_dtype == SLOKV_DTYPE_BF16 ? go(int4_rows_widen_kernel<__nv_bfloat16>, __nv_bfloat16())
                                        : go(int4_rows_widen_kernel<__half>, __half());
+}
+
+extern "C" int slokv_int4_rows_expand(const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                      int32_t num_rows, int32_t num_tokens, int32_t *table_rows,
+                                      int32_t *context_lens, void *stream) {
+  using namespace slokv;
+  if (num_rows < 0 || num_tokens < 0) return SLOKV_ERR_INVALID_ARG;
+  if (num_rows == 0 || num_tokens == 0) return SLOKV_OK;
+  if (!cu_seqlens_q || !cu_seqlens_k || !table_rows || !context_lens) return SLOKV_ERR_INVALID_ARG;
+  int4_rows_expand_kernel<<<static_cast<unsigned>((num_tokens + 127ll) / 128), 128, 0,
+                            static_cast<cudaStream_t>(stream)>>>(
+      cu_seqlens_q, cu_seqlens_k, num_rows, num_tokens, table_rows, context_lens);
+  return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
 }

@@ -5,7 +5,9 @@
 // x and lse are the log2-domain scores and denominators that the decode kernels store
 // (4 G bytes a token and head against the K and V rows' 144 to 512, so that K is not
 // read a second time).  One thread takes four tokens of one head and adds its group
-// in order: no atomics, the same sum on every run.
+// in order: no atomics, the same sum on every run.  The bf16 / f16 decode stores a row of
+// tokens per head, the 4-bit decode the heads of a token side by side (what their
+// accumulators make contiguous); both are read here.
 #include "common.cuh"
 
 namespace slokv {
@@ -34,8 +36,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// kVec: score and logit rows allow 16-byte accesses.
-template <bool kVec>
+// kPairs: logits are [batch, hkv, logits_stride, group padded to even]; else [batch, hq,
+// logits_stride], and kVec: score and logit rows allow 16-byte accesses.
+template <bool kPairs, bool kVec>
 __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const ScoreParams p) {
   const int32_t b = blockIdx.z, h = blockIdx.y;
   int32_t len = __ldg(p.lens + b);
@@ -49,41 +52,71 @@ __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const Sc
     if (first) record_error(p.err, SLOKV_DEVERR_CONTEXT_LEN);
     len = p.cap;
   }
-  const int32_t t = (blockIdx.x * kThreads + threadIdx.x) * kPer;
-  if (t >= len) return;
-  const int32_t n = min(kPer, len - t);
-  const float *lg =
-      p.logits + (static_cast<int64_t>(b) * p.hkv + h) * p.group * p.logits_stride + t;
-  const float *lse = p.lse + (static_cast<int64_t>(b) * p.hkv + h) * p.group;
-  float w[kPer] = {0.f, 0.f, 0.f, 0.f};
-  for (int g = 0; g < p.group; ++g, lg += p.logits_stride) {
-    const float d = __ldg(lse + g);
-    if (d == -INFINITY) continue;  // a head whose every score is -inf has no weights
-    float x[kPer];
-    if (kVec && n == kPer) {
-      const float4 v = __ldg(reinterpret_cast<const float4 *>(lg));
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = i < n ? __ldg(lg + i) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) w[i] += exp2_fast(x[i] - d);
-  }
-  float *s = p.scores + row * p.row_stride + h * p.head_stride + t;
-  if (kVec && n == kPer) {
+  const int64_t pair = static_cast<int64_t>(b) * p.hkv + h;
+  const float *lse = p.lse + pair * p.group;
+  float *score = p.scores + row * p.row_stride + h * p.head_stride;
+  if constexpr (kPairs) {
+    // a warp's lanes take neighbouring tokens, whose heads lie side by side
+    const int32_t heads = (p.group + 1) / 2 * 2;
+    const int32_t t0 = blockIdx.x * kThreads * kPer + threadIdx.x;
+    if (t0 >= len) return;
+    const float *lg = p.logits + (pair * p.logits_stride + t0) * heads;
+    const int64_t step = static_cast<int64_t>(kThreads) * heads;
+    float w[kPer] = {0.f, 0.f, 0.f, 0.f}, before[kPer] = {0.f, 0.f, 0.f, 0.f};
     if (p.decay != 0.f) {
-      const float4 v = *reinterpret_cast<const float4 *>(s);
-      w[0] = fmaf(p.decay, v.x, w[0]);
-      w[1] = fmaf(p.decay, v.y, w[1]);
-      w[2] = fmaf(p.decay, v.z, w[2]);
-      w[3] = fmaf(p.decay, v.w, w[3]);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (t0 + i * kThreads < len) before[i] = score[t0 + i * kThreads];
     }
-    *reinterpret_cast<float4 *>(s) = make_float4(w[0], w[1], w[2], w[3]);
-  } else {
+#pragma unroll 2
+    for (int g = 0; g < p.group; g += 2) {
+      // a head whose every score is -inf has no weights; nor has the padding
+      const float d0 = __ldg(lse + g), d1 = g + 1 < p.group ? __ldg(lse + g + 1) : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (t0 + i * kThreads < len) {
+          const float2 x = __ldg(reinterpret_cast<const float2 *>(lg + i * step + g));
+          if (d0 != -INFINITY) w[i] += exp2_fast(x.x - d0);
+          if (d1 != -INFINITY) w[i] += exp2_fast(x.y - d1);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (i < n) s[i] = p.decay != 0.f ? fmaf(p.decay, s[i], w[i]) : w[i];
+      if (t0 + i * kThreads < len) score[t0 + i * kThreads] = fmaf(p.decay, before[i], w[i]);
+    return;
+  } else {
+    const int32_t t = (blockIdx.x * kThreads + threadIdx.x) * kPer;
+    if (t >= len) return;
+    const int32_t n = min(kPer, len - t);
+    float w[kPer] = {0.f, 0.f, 0.f, 0.f};
+    const float *lg = p.logits + pair * p.group * p.logits_stride + t;
+    float4 before = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (kVec && n == kPer && p.decay != 0.f) before = *reinterpret_cast<const float4 *>(score + t);
+#pragma unroll 4
+    for (int g = 0; g < p.group; ++g, lg += p.logits_stride) {
+      const float d = __ldg(lse + g);
+      if (d == -INFINITY) continue;
+      float x[kPer];
+      if (kVec && n == kPer) {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(lg));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] = i < n ? __ldg(lg + i) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) w[i] += exp2_fast(x[i] - d);
+    }
+    float *s = score + t;
+    if (kVec && n == kPer) {
+      *reinterpret_cast<float4 *>(s) =
+          make_float4(fmaf(p.decay, before.x, w[0]), fmaf(p.decay, before.y, w[1]),
+                      fmaf(p.decay, before.z, w[2]), fmaf(p.decay, before.w, w[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < n) s[i] = p.decay != 0.f ? fmaf(p.decay, s[i], w[i]) : w[i];
+    }
   }
 }
 
@@ -93,8 +126,8 @@ __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const Sc
 extern "C" int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int64_t head_stride,
                                           int32_t width, int32_t num_score_rows,
                                           const int32_t *score_rows, const float *logits,
-                                          int64_t logits_stride, const float *lse,
-                                          const int32_t *context_lens, int32_t batch,
+                                          int64_t logits_stride, int32_t logits_pairs,
+                                          const float *lse, const int32_t *context_lens, int32_t batch,
                                           int32_t num_q_heads, int32_t num_kv_heads,
                                           int64_t max_context, float decay, uint32_t *dev_error,
                                           void *stream) {
@@ -132,9 +165,11 @@ extern "C" int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int
   const dim3 grid(static_cast<unsigned>((cap + kThreads * kPer - 1) / (kThreads * kPer)),
                   static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (vec)
-    kv_scores_accumulate_kernel<true><<<grid, kThreads, 0, st>>>(p);
+  if (logits_pairs && (reinterpret_cast<uintptr_t>(logits) & 7u)) return SLOKV_ERR_ALIGNMENT;
+  auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, st>>>(p); };
+  if (logits_pairs)
+    go(kv_scores_accumulate_kernel<true, false>);
   else
-    kv_scores_accumulate_kernel<false><<<grid, kThreads, 0, st>>>(p);
+    vec ? go(kv_scores_accumulate_kernel<false, true>) : go(kv_scores_accumulate_kernel<false, false>);
   return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
 }

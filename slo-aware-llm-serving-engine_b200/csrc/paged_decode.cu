@@ -451,14 +451,24 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
         const int64_t pos = static_cast<int64_t>(j) * kTile;
         const int64_t room = min(static_cast<int64_t>(valid), p.logits_stride - pos);
         float *lg = p.logits + (static_cast<int64_t>(r.b) * p.hkv * G + r.h * G + g) * p.logits_stride + pos;
+        if (room >= kTile) {
+          // rows are a multiple of four floats apart, so a pair is one 8-byte store
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-          for (int e2 = 0; e2 < 2; ++e2) {
-            const int tok = nt * 8 + 2 * c + e2;
-            if (tok < room && g < G) lg[tok] = sc[nt][e2];
-            if (tok < room && g + 8 < G) lg[8 * p.logits_stride + tok] = sc[nt][2 + e2];
+          for (int nt = 0; nt < 4; ++nt) {
+            float2 *at = reinterpret_cast<float2 *>(lg + nt * 8 + 2 * c);
+            if (g < G) *at = make_float2(sc[nt][0], sc[nt][1]);
+            if (g + 8 < G) at[4 * p.logits_stride] = make_float2(sc[nt][2], sc[nt][3]);
           }
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              const int tok = nt * 8 + 2 * c + e2;
+              if (tok < room && g < G) lg[tok] = sc[nt][e2];
+              if (tok < room && g + 8 < G) lg[8 * p.logits_stride + tok] = sc[nt][2 + e2];
+            }
+        }
       }
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
@@ -1121,6 +1131,7 @@ extern "C" int slokv_paged_decode_logits(void *out, int64_t out_stride_b, int64_
                                          size_t workspace_bytes, uint32_t *dev_error,
                                          void *stream) {
   if (batch > 0 && (!logits || !lse || logits_stride <= 0)) return SLOKV_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(logits) & 15u) || (logits_stride & 3)) return SLOKV_ERR_ALIGNMENT;
   return slokv::decode::run_decode(
       false, out, out_stride_b, out_stride_h, q, q_stride_b, q_stride_h, k_cache, v_cache,
       k_block_stride, v_block_stride, nullptr, nullptr, num_blocks, block_size, num_q_heads,

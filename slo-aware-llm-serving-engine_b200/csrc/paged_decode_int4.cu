@@ -87,9 +87,11 @@ struct Params {
   float *partials;                    // [nslots][2][group][kRowFloats]
   int4 *jobs;                         // [nslots]: segment (b, h, first slot, last slot) of the warp
                                       // slot's head partial (x = -1: it has none)
-  float *logits;                      // scored: [batch, hq, logits_stride] log2-domain scores
+  const int32_t *table_rows;          // table row of each sequence, or null: its own index
+  float *logits;                      // scored: [batch, hkv, logits_stride, logits_heads] log2-
+                                      // domain scores (logits_heads: the group, padded to even)
   float *lse;                         // scored: [batch, hq] log2 of the softmax denominator
-  int64_t logits_stride;
+  int32_t logits_stride, logits_heads;
   uint32_t *err;
   int32_t nslots;
 };
@@ -252,6 +254,7 @@ struct Cursor {
 };
 
 __device__ __forceinline__ int32_t table_entry(const Params &p, int32_t b, int32_t page) {
+  if (p.table_rows) b = __ldg(p.table_rows + b);
   return __ldg(p.block_tables + static_cast<int64_t>(b) * p.bt_stride + page);
 }
 
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
     const int32_t len = __ldg(p.context_lens + b);
     if (len > static_cast<int64_t>(p.max_blocks) * p.block_size && threadIdx.x == 0)
       record_error(p.err, SLOKV_DEVERR_CONTEXT_LEN);
-    if (len > 0) continue;
+    if (len > 0 || (len < 0 && p.table_rows)) continue;  // (expanded rows: -1 is not ours to write)
     T *ob = static_cast<T *>(p.out) + static_cast<int64_t>(b) * p.out_sb;
     for (int i = threadIdx.x; i < p.hkv * G * kD; i += blockDim.x) {
       const int row = i / kD, d = i - row * kD;
@@ -525,6 +528,14 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
         __syncwarp();
       }
 
+      float *lg = nullptr;
+      int room = 0;
+      if constexpr (kScored) {
+        room = min(valid, p.logits_stride - j * kTile);
+        lg = p.logits + ((static_cast<int64_t>(r.b) * p.hkv + r.h) * p.logits_stride + j * kTile) * p.logits_heads +
+             2 * c;
+      }
+
       // ---- scores of 64 tokens x 8 kN heads, in the accumulators' unit ----
       float sc[kN][4][4];
 #pragma unroll
@@ -567,6 +578,15 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
             for (int x = 0; x < 2; ++x)
               sc[rr][i][2 * row + x] = fmaf(s0, acc[rr][0][2 * row + x],
                                             fmaf(s1, acc[rr][1][2 * row + x], sc[rr][i][2 * row + x]));
+          if constexpr (kScored) {
+            // head pairs innermost: the lanes of 8 tokens write one contiguous run
+            const int tok = 16 * i + 8 * row + tok_k;
+#pragma unroll
+            for (int rr = 0; rr < kN; ++rr)
+              if (tok < room && 8 * rr + 2 * c < G)
+                *reinterpret_cast<float2 *>(lg + tok * p.logits_heads + 8 * rr) =
+                    make_float2(sc[rr][i][2 * row] * unscale[rr][0], sc[rr][i][2 * row + 1] * unscale[rr][1]);
+          }
         }
       }
       if (valid < kTile) {
@@ -579,27 +599,6 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
               for (int rr = 0; rr < kN; ++rr) sc[rr][i][2 * row] = sc[rr][i][2 * row + 1] = -INFINITY;
             }
       }
-      if constexpr (kScored) {
-        const int64_t pos = static_cast<int64_t>(j) * kTile;
-        const int64_t room = min(static_cast<int64_t>(valid), p.logits_stride - pos);
-#pragma unroll
-        for (int rr = 0; rr < kN; ++rr)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int head = 8 * rr + 2 * c + x;
-            if (head >= G) continue;
-            float *lg = p.logits +
-                        (static_cast<int64_t>(r.b) * p.hkv * G + r.h * G + head) * p.logits_stride + pos;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int row = 0; row < 2; ++row) {
-                const int tok = 16 * i + 8 * row + tok_k;
-                if (tok < room) lg[tok] = sc[rr][i][2 * row + x] * unscale[rr][x];
-              }
-          }
-      }
-
       // ---- online softmax ----
       {
         // positive bf16 order as their bits, and both halves of a word count
@@ -942,8 +941,9 @@ extern "C" int slokv_paged_decode_int4(void *out, int64_t out_stride_b, int64_t 
                                        int32_t num_q_heads, int32_t num_kv_heads,
                                        int32_t head_dim, const int32_t *block_tables,
                                        int64_t block_table_stride, int32_t max_blocks_per_seq,
-                                       const int32_t *context_lens, int32_t batch,
-                                       float softmax_scale, int32_t q_dtype, float *logits,
+                                       const int32_t *table_rows, const int32_t *context_lens,
+                                       int32_t batch, float softmax_scale, int32_t q_dtype,
+                                       float *logits,
                                        int64_t logits_stride, float *lse, void *workspace,
                                        size_t workspace_bytes, uint32_t *dev_error,
                                        void *stream) {
@@ -960,7 +960,8 @@ extern "C" int slokv_paged_decode_int4(void *out, int64_t out_stride_b, int64_t 
   if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens ||
       max_blocks_per_seq <= 0 || (logits != nullptr) != (lse != nullptr))
     return SLOKV_ERR_INVALID_ARG;
-  if (logits && logits_stride <= 0) return SLOKV_ERR_INVALID_ARG;
+  if (logits && (logits_stride <= 0 || logits_stride > 0x7fffffff)) return SLOKV_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(logits) & 7u) return SLOKV_ERR_ALIGNMENT;
   const int64_t run = static_cast<int64_t>(num_kv_heads) * block_size * kRowBytes;
   if (((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15u) ||
       ((k_block_stride | v_block_stride) & 15) || k_block_stride < run || v_block_stride < run)
@@ -998,9 +999,11 @@ extern "C" int slokv_paged_decode_int4(void *out, int64_t out_stride_b, int64_t 
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.partials = static_cast<float *>(workspace);
   p.jobs = reinterpret_cast<int4 *>(static_cast<char *>(workspace) + partial_bytes_for(sms, group));
+  p.table_rows = table_rows;
   p.logits = logits;
+  p.logits_heads = (group + 1) / 2 * 2;
   p.lse = lse;
-  p.logits_stride = logits_stride;
+  p.logits_stride = static_cast<int32_t>(logits_stride);
   p.err = dev_error;
   p.nslots = sms * warps_for(group);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

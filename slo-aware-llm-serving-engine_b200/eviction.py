@@ -121,13 +121,15 @@ def flash_attn_with_kvcache_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cac
                                                                                     Hkv)
         # one scratch: the decode's workspace, the scores of this step, their denominators
         logits_at = (nbytes + 255) // 256 * 256
-        lse_at = logits_at + 4 * B * Hq * stride
+        # (the 4-bit decode stores a KV head's heads side by side, padded to pairs)
+        heads = Hkv * ((Hq // Hkv + 1) // 2 * 2) if four else Hq
+        lse_at = logits_at + 4 * B * heads * stride
         scratch = torch.empty(lse_at + 4 * B * Hq, dtype=torch.uint8, device=dev)
         ws = scratch.data_ptr()
         logits, lse, err = ws + logits_at, ws + lse_at, buffers.error_word(dev).data_ptr()
         if four:
-            launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens, block_table, scale, B, Hq,
-                               out, ws, nbytes, err, stream, logits, stride, lse)
+            launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens.data_ptr(), block_table,
+                               scale, B, Hq, out, ws, nbytes, err, stream, logits, stride, lse)
         else:
             qs, os = q.stride(), out.stride()
             check(lib().slokv_paged_decode_logits(
@@ -137,7 +139,7 @@ def flash_attn_with_kvcache_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cac
                 cache_seqlens.data_ptr(), B, scale, _DECODE_DTYPES[q.dtype], logits, stride, lse, ws,
                 nbytes, err, stream), "paged_decode_logits")
         check(lib().slokv_kv_scores_accumulate(
-            scores.data_ptr(), row, head, width, rows, rows_ptr, logits, stride, lse,
+            scores.data_ptr(), row, head, width, rows, rows_ptr, logits, stride, int(four), lse,
             cache_seqlens.data_ptr(), B, Hq, Hkv, block_table.shape[1] * bs, float(decay), err,
             stream), "kv_scores_accumulate")
     return out

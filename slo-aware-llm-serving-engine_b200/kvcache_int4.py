@@ -26,6 +26,13 @@ TILE_TOKENS = 64
 ROW_BYTES = 72          # 64 bytes of codes, 2 x (scale, minimum) in bf16
 _WIDE_PAGE = 128        # tokens of a page that rows are widened to for prefill
 
+# A prefill call of at most SHORT_CHUNK query tokens a row, or SHORT_CALL in all, runs as
+# decode rows (8 KV heads of 4, us, prefill / decode rows, L cached tokens: 1 row of 64
+# on L 4000 82 / 63, of 128 79 / 110; 8 rows of 16 115 / 109, of 32 113 / 202; 64 rows
+# of 4 793 / 204, of 16 783 / 783).
+SHORT_CHUNK, SHORT_CALL = 16, 64
+_MAX_DECODE_ROWS = 8192
+
 _Q_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _STORE_DTYPES = {**_Q_DTYPES, torch.float32: _lib.DTYPE_F32}
 
@@ -160,15 +167,17 @@ def decode_int4_workspace_bytes(index: int, num_q_heads: int, num_kv_heads: int)
     return n
 
 
-def launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens, block_table, scale, B, Hq, out,
-                       workspace, nbytes, err, stream, logits=None, logits_stride=0, lse=None):
-    """slokv_paged_decode_int4 on checked arguments; workspace, logits and lse are addresses."""
+def launch_decode_int4(q, k_cache, v_cache, pool, lens, block_table, scale, B, Hq, out, workspace,
+                       nbytes, err, stream, logits=None, logits_stride=0, lse=None,
+                       table_rows=None):
+    """slokv_paged_decode_int4 on checked arguments; lens, workspace, logits, lse and
+    table_rows are addresses; q / out [B, ..., Hq, 128]."""
     NB, bs, Hkv, k_block, v_block = pool
     qs, os = q.stride(), out.stride()
     check(lib().slokv_paged_decode_int4(
-        out.data_ptr(), os[0], os[2], q.data_ptr(), qs[0], qs[2], k_cache.data_ptr(),
+        out.data_ptr(), os[0], os[-2], q.data_ptr(), qs[0], qs[-2], k_cache.data_ptr(),
         v_cache.data_ptr(), k_block, v_block, NB, bs, Hq, Hkv, HEAD_DIM, block_table.data_ptr(),
-        block_table.stride(0), block_table.shape[1], cache_seqlens.data_ptr(), B, scale,
+        block_table.stride(0), block_table.shape[1], table_rows, lens, B, scale,
         _Q_DTYPES[q.dtype], logits, logits_stride, lse, workspace, nbytes, err, stream),
         "paged_decode_int4")
 
@@ -192,8 +201,8 @@ def flash_attn_with_kvcache_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache
     with on_device(dev) as stream:
         nbytes = decode_int4_workspace_bytes(dev.index, Hq, pool[2])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens, block_table, scale, B, Hq, out,
-                           ws.data_ptr(), nbytes, buffers.error_word(dev).data_ptr(), stream)
+        launch_decode_int4(q, k_cache, v_cache, pool, cache_seqlens.data_ptr(), block_table, scale,
+                           B, Hq, out, ws.data_ptr(), nbytes, buffers.error_word(dev).data_ptr(), stream)
     return out
 
 
@@ -203,10 +212,10 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
     """Causal varlen attention over a 4-bit pool's pages (block_table required).
 
     Arguments as flash_attn_varlen_func's paged form, any block_size that the pool
-    allows.  The rows' cached tokens are widened once to q's type (one rounding) in a
-    scratch of rows x ceil(max_seqlen_k / 128) pages, which the tcgen05 prefill then
-    reads: 16 times the prefill's own page reads at most when a chunk is a few
-    tokens, a few per cent of its time when it is a thousand.
+    allows.  Short calls (SHORT_CHUNK, SHORT_CALL) run as decode rows, one a query
+    token.  For longer ones the rows' cached tokens are widened once to q's type (one
+    rounding) in a scratch of rows x ceil(max_seqlen_k / 128) pages, which the tcgen05
+    prefill then reads: a few per cent of its time when a chunk is a thousand tokens.
     """
     if block_table is None:
         raise SlokvError("4-bit varlen attention reads the pool: block_table is required")
@@ -216,7 +225,8 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
             or q.stride(-1) != 1:
         raise SlokvError(f"q must be bf16/f16 [tokens, heads, {HEAD_DIM}] with a contiguous last "
                          "dim")
-    NB, bs, Hkv, k_block, v_block = int4_geometry(k_cache, v_cache)
+    pool = int4_geometry(k_cache, v_cache)
+    NB, bs, Hkv, k_block, v_block = pool
     dev = require_cuda(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, out)
     _i32_contig("cu_seqlens_q", cu_seqlens_q)
     _i32_contig("cu_seqlens_k", cu_seqlens_k)
@@ -226,13 +236,28 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(-1) != 1 \
             or block_table.shape[0] < rows:
         raise SlokvError("block_table must be int32 [rows, pages] with a contiguous last dim")
-    if q.shape[1] % Hkv:
+    Tq, Hq, _ = q.shape
+    if Hq % Hkv:
         raise SlokvError("query heads must divide by the KV heads")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != q.shape or out.stride(-1) != 1:
         raise SlokvError("out must match q's shape and dtype with a contiguous last dim")
-    if q.shape[0] == 0 or rows <= 0 or int(max_seqlen_q) <= 0:
+    if Tq == 0 or rows <= 0 or int(max_seqlen_q) <= 0:
+        return out
+    if ((max_seqlen_q <= SHORT_CHUNK or Tq <= SHORT_CALL) and Tq <= _MAX_DECODE_ROWS
+            and block_table.shape[1]):
+        scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
+        with on_device(dev) as stream:
+            nbytes = decode_int4_workspace_bytes(dev.index, Hq, Hkv)
+            ws = torch.empty(nbytes + 8 * Tq, dtype=torch.uint8, device=dev)
+            table_rows, lens = ws.data_ptr() + nbytes, ws.data_ptr() + nbytes + 4 * Tq
+            check(lib().slokv_int4_rows_expand(cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+                                               rows, Tq, table_rows, lens, stream),
+                  "int4_rows_expand")
+            launch_decode_int4(q, k_cache, v_cache, pool, lens, block_table, scale, Tq, Hq, out,
+                               ws.data_ptr(), nbytes, buffers.error_word(dev).data_ptr(), stream,
+                               table_rows=table_rows)
         return out
     pages = max(1, (int(max_seqlen_k) + _WIDE_PAGE - 1) // _WIDE_PAGE)
     with on_device(dev) as stream:

@@ -386,9 +386,12 @@ def test_decode_captured_twice_and_other_stream(pkg):
     ([33, 257], [1000, 127], 2, 2, 256, torch.float16),
     ([64], [2049], 8, 4, 128, torch.bfloat16),
     ([7, 0, 12], [9, 100, 500], 1, 1, 64, torch.float16),
+    ([16] * 5, [0, 0, 300, 63, 64], 2, 8, 64, torch.bfloat16),
+    ([17] * 5, [0, 0, 300, 63, 64], 2, 8, 64, torch.bfloat16),
 ])
 def test_varlen(pkg, qlens, hist, H, G, bs, dtype):
-    """Against fp64 attention on the pool's values rounded to q's type (the documented
+    """Short calls (SHORT_CHUNK, SHORT_CALL) run as decode rows and have their bound.  Longer
+    ones: against fp64 attention on the pool's values rounded to q's type (the documented
     rounding).  Bound: a rounded probability (half a step of the type, relative) and a
     rounded output, 2 half-steps of sum w |v|, plus the fp32 scores' 400 u of their absolute
     sum as above and the exponential, in all below 2^-13 of sum w |v|."""
@@ -413,6 +416,13 @@ def test_varlen(pkg, qlens, hist, H, G, bs, dtype):
     out = pkg.flash_attn_varlen_func_int4(q.cuda(), kp, vp, cu(qlens).cuda(), cu(klens).cuda(),
                                           max(qlens), max(klens), block_table=tables.cuda()).cpu()
     assert pkg.read_device_errors() == 0
+    from importlib import import_module
+    K = import_module("slo-aware-llm-serving-engine_b200.kvcache_int4")
+    if max(qlens) <= K.SHORT_CHUNK or sum(qlens) <= K.SHORT_CALL:
+        seen = [nk - nq + i + 1 for nq, nk in zip(qlens, klens) for i in range(nq)]
+        per = torch.cat([tables[b:b + 1].expand(nq, -1) for b, nq in enumerate(qlens)])
+        check_decode(out.unsqueeze(1), q.unsqueeze(1), kp, vp, seen, per, 128 ** -0.5)
+        return
     kv, vv = R.decode_pool(kp.cpu())[0], R.decode_pool(vp.cpu())[0]
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
     at = 0
@@ -427,15 +437,34 @@ def test_varlen(pkg, qlens, hist, H, G, bs, dtype):
         at += nq
 
 
-def test_varlen_bad_metadata_is_flagged(pkg):
+@pytest.mark.parametrize("nq", [2, 70])
+def test_varlen_bad_metadata_is_flagged(pkg, nq):
     kp, vp = make_pool(pkg, 95, 4, 64, 1), make_pool(pkg, 96, 4, 64, 1)
-    q = torch.zeros(2, 2, 128, dtype=torch.bfloat16, device="cuda")
-    cu_q = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    q = torch.zeros(nq, 2, 128, dtype=torch.bfloat16, device="cuda")
+    cu_q = torch.tensor([0, nq], dtype=torch.int32, device="cuda")
     cu_k = torch.tensor([0, 100], dtype=torch.int32, device="cuda")
     pkg.read_device_errors()
-    out = pkg.flash_attn_varlen_func_int4(q, kp, vp, cu_q, cu_k, 2, 100, block_table=torch.tensor(
+    out = pkg.flash_attn_varlen_func_int4(q, kp, vp, cu_q, cu_k, nq, 100, block_table=torch.tensor(
         [[1, 9]], dtype=torch.int32, device="cuda"))
     assert pkg.read_device_errors() & 0x2 and torch.isfinite(out).all()
-    pkg.flash_attn_varlen_func_int4(q, kp, vp, cu_q, cu_k, 2, 100, block_table=torch.tensor(
+    pkg.flash_attn_varlen_func_int4(q, kp, vp, cu_q, cu_k, nq, 100, block_table=torch.tensor(
         [[1]], dtype=torch.int32, device="cuda"))
     assert pkg.read_device_errors() & 0x4
+
+
+@pytest.mark.parametrize("nq", [3, 66])
+def test_varlen_rows_behind_and_without_keys(pkg, nq):
+    """Query tokens before the first and behind the last row keep what `out` held; a query that
+    sees no key (more queries than keys) gives zeros."""
+    H, G, bs = 1, 2, 64
+    kp, vp = make_pool(pkg, 97, 4, bs, H), make_pool(pkg, 98, 4, bs, H)
+    q = torch.from_numpy(det_normal(99, (nq + 7, 2, 128))).float().bfloat16()
+    out = torch.full((nq + 7, 2, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    pkg.read_device_errors()
+    pkg.flash_attn_varlen_func_int4(q.cuda(), kp, vp, torch.tensor([0, nq], dtype=torch.int32).cuda(),
+                                    torch.tensor([0, nq - 2], dtype=torch.int32).cuda(), nq, nq - 2,
+                                    block_table=torch.tensor([[3]], dtype=torch.int32).cuda(), out=out)
+    assert pkg.read_device_errors() == 0
+    assert (out[nq:] == 5).all() and (out[:2] == 0).all()
+    check_decode(out[2:nq].unsqueeze(1), q[2:nq].unsqueeze(1), kp, vp, list(range(1, nq - 1)),
+                 torch.full((nq, 1), 3), 128 ** -0.5) if nq <= 32 else None

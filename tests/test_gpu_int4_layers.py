@@ -64,12 +64,12 @@ def test_attention_prefill_decode_mixed(pkg):
         assert torch.equal(vv[s // bs, s % bs], wv[s // bs, s % bs])
 
     # a chunk with cached history
-    q, k, v = rows(11, 60, H, G)
-    slots = [slot(0, 100 + t) for t in range(40)] + [slot(1, 50 + t) for t in range(20)]
-    pkg.set_context(True, cu([40, 20]), cu([140, 70]), 40, 140, i32(slots), None, tables.cuda())
+    q, k, v = rows(11, 70, H, G)
+    slots = [slot(0, 90 + t) for t in range(50)] + [slot(1, 50 + t) for t in range(20)]
+    pkg.set_context(True, cu([50, 20]), cu([140, 70]), 50, 140, i32(slots), None, tables.cuda())
     out = attn(q, k, v)
     pkg.reset_context()
-    check_varlen(out, q, *values(), tables, [40, 20], [140, 70])
+    check_varlen(out, q, *values(), tables, [50, 20], [140, 70])
 
     # a decode step, not scored and scored: the same outputs
     q, k, v = rows(12, 2, H, G)
@@ -96,7 +96,8 @@ def test_attention_prefill_decode_mixed(pkg):
     pkg.reset_context()
     check_decode(out[:1].unsqueeze(1), q[:1].unsqueeze(1).cpu(), attn.k_cache, attn.v_cache, [142], tables,
                  128 ** -0.5)
-    check_varlen(out[1:], q[1:], *values(), tables[1:], [30], [101])
+    check_decode(out[1:].unsqueeze(1), q[1:].unsqueeze(1).cpu(), attn.k_cache, attn.v_cache,
+                 list(range(72, 102)), tables[1:].expand(30, -1), 128 ** -0.5)
     assert ((attn.scores[1].sum(-1).cpu() - G).abs() < G * 2.0 ** -16).all()
     assert pkg.read_device_errors() == 0
 

@@ -47,8 +47,8 @@ def test_decode_int4_arguments(pkg):
     def call(hq=8, hkv=2, d=128, bs=64, dt=0, batch=3, q=P, cache=P, stride=2 * 64 * 72, osb=1024,
              logits=None, lse=None, ls=0, w=4):
         return lib.slokv_paged_decode_int4(P, osb, 128, q, 1024, 128, cache, cache, stride, stride, 3, bs,
-                                           hq, hkv, d, P, 4, w, P, batch, 0.1, dt, logits, ls, lse,
-                                           None, 0, None, None)
+                                           hq, hkv, d, P, 4, w, None, P, batch, 0.1, dt, logits, ls,
+                                           lse, None, 0, None, None)
     assert call(batch=0) == 0 and call(batch=-1) == -1
     assert call(batch=8193) == -3 and call(d=64) == -3 and call(dt=2) == -3
     assert call(hq=7) == -1 and call(hq=34) == -3 and call(bs=96) == -3
@@ -56,6 +56,9 @@ def test_decode_int4_arguments(pkg):
     assert call(logits=P) == -1 and call(logits=P, lse=P, ls=0) == -1
     assert call(cache=ctypes.c_void_p(264)) == -2 and call(stride=2 * 64 * 72 + 4) == -2
     assert call(q=ctypes.c_void_p(258)) == -2 and call(osb=1023) == -2
+    assert call(logits=ctypes.c_void_p(260), lse=P, ls=64) == -2
+    ex = lambda r=1, t=1, a=P: lib.slokv_int4_rows_expand(a, P, r, t, P, P, None)
+    assert ex(r=0) == 0 and ex(t=0) == 0 and ex(r=-1) == -1 and ex(t=-1) == -1 and ex(a=None) == -1
     assert lib.slokv_paged_decode_int4_workspace_bytes(0, 7, 2, 128) == 0
     assert lib.slokv_paged_decode_int4_workspace_bytes(0, 8, 2, 64) == 0
     assert lib.slokv_paged_decode_int4_workspace_bytes(0, 34, 2, 128) == 0
@@ -68,12 +71,13 @@ def test_logits_and_scores_arguments(pkg):
         return lib.slokv_paged_decode_logits(P, 1024, 128, P, 1024, 128, P, P, 32768, 32768, 3, 64, 8, 2,
                                              128, P, 4, 4, P, 3, 0.1, dt, lg, ls, lse, None, 0, None, None)
     assert logits(lg=None) == -1 and logits(lse=None) == -1 and logits(ls=0) == -1
+    assert logits(ls=66) == -2 and logits(lg=ctypes.c_void_p(264)) == -2
     assert logits(dt=2) == -3                              # fp32 pools are not scored
     assert logits(dt=3) == -3
 
     def acc(batch=2, hq=8, hkv=2, width=64, scores=P, rows=2, cap=256, ls=64):
-        return lib.slokv_kv_scores_accumulate(scores, 128, 64, width, rows, None, P, ls, P, P, batch, hq,
-                                              hkv, cap, 1.0, None, None)
+        return lib.slokv_kv_scores_accumulate(scores, 128, 64, width, rows, None, P, ls, 0, P, P, batch,
+                                              hq, hkv, cap, 1.0, None, None)
     assert acc(batch=0) == 0 and acc(width=0) == 0 and acc(cap=0) == 0
     assert acc(batch=-1) == -1 and acc(hq=7) == -1 and acc(scores=None) == -1 and acc(ls=0) == -1
     assert acc(batch=65536) == -3 and acc(scores=ctypes.c_void_p(258)) == -2
