@@ -10,17 +10,21 @@
 // parameters are its own, so nothing stored before is touched and a page needs no
 // reset when it changes hands.
 //
-// Append: half a warp per row of 128 dims, 8 dims a lane: one 16-byte load, a three-step
-// shuffle min / max over the 8 lanes of a group, one 32-bit word of codes stored (the half
-// warp's words are the row's 64 contiguous bytes).  A CTA takes 8 tokens of one head, K
-// and V, so its rows are neighbours in the page.  The quotient is a multiplication by
-// 1 / scale, 2^-23 of itself off; where that leaves it within 2^-12 of a border between
-// two codes the lane divides, so the codes are those of the true division.
+// Append: eight lanes per row of 128 dims, 16 dims a lane: two 16-byte loads, a two-step
+// shuffle min / max over the 4 lanes of a group, one exchange between the groups' lanes and an
+// 8-byte store (the eight lanes' stores are the row's 64 contiguous bytes).  A CTA takes 16
+// tokens of one head, K and V, so its rows are neighbours in the page.  Issue-bound (31 us
+// for 6211 tokens of 8 heads with a division a value and 8 dims a lane), so the quotient
+// is a multiplication by an approximate 1 / scale, 2^-22 of itself off; a value that this
+// leaves within 2^-16 of a border between two codes is divided, and the codes are
+// always those of the true division.
 //
 // Read-back and widening: eight lanes per row, each with the 8 bytes that hold 8 dims
 // of either group, so that the 16-byte stores of a row are contiguous.
 #include "common.cuh"
 #include "int4_page.cuh"
+
+#include <type_traits>
 
 namespace slokv {
 namespace {
@@ -28,7 +32,7 @@ namespace {
 using namespace kv4;
 
 constexpr int kThreads = 256;
-constexpr int kRowsPerCta = kThreads / 16;
+constexpr int kRowsPerCta = kThreads / 8;
 
 template <typename T>
 __device__ __forceinline__ float widen(T x);
@@ -41,7 +45,7 @@ __device__ __forceinline__ float widen<float>(float x) { return x; }
 
 // Eight consecutive elements of a row; kVec: the address is 16-byte aligned.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
+__device__ __forceinline__ void load8(const T *p, float *x) {
   if constexpr (kVec && sizeof(T) == 2) {
     const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p));
     const T *e = reinterpret_cast<const T *>(&raw);
@@ -58,30 +62,49 @@ __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
   }
 }
 
-// Codes of 8 values of a group with minimum m and scale s > 0, the k-th in bits 4k ..
-__device__ __forceinline__ uint32_t encode8(const float (&x)[8], float m, float s) {
-  const float inv = __fdiv_rn(1.f, s);
-  const float magic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
+// n / d for 0 <= n < 2^31 without a division (the round-up method of Granlund and
+// Montgomery, 1994): q = (n + high32(n m)) >> l with l = ceil(log2 d) and
+// m = floor(2^32 (2^l - d) / d) + 1.
+struct FastDiv {
+  uint32_t m, l;
+  explicit FastDiv(uint32_t d) {
+    l = 0;
+    while ((1ull << l) < d) ++l;
+    m = static_cast<uint32_t>((((1ull << l) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int32_t operator()(int32_t n) const {
+    const uint32_t u = static_cast<uint32_t>(n);
+    return static_cast<int32_t>((u + __umulhi(u, m)) >> l);
+  }
+};
+
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Codes of 8 values of a group with minimum m and scale s > 0, the k-th in bits 4k ..;
+// inv: 1 / s, approximately.  kExact: m is the minimum itself, so x >= m, and s >= range /
+// 15 (1 - 2^-8) gives quotients below 15.1: no code needs clamping.  (Scales below 2^-120,
+// which bf16 may hold less exactly, always divide: inv is NaN for them.  None is above
+// 2^125, so the reciprocal is a normal number.)
+template <bool kExact>
+__device__ __forceinline__ uint32_t encode8(const float *x, float m, float s, float inv) {
+  const float magic = 12582912.f;    // 1.5 * 2^23: adding it rounds to an integer
   uint32_t word = 0;
-  bool near = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 7; i >= 0; --i) {
     const float d = __fsub_rn(x[i], m);
     const float t = __fmaf_rn(d, inv, magic);
-    const float off = __fmaf_rn(d, inv, -__fsub_rn(t, magic));
-    near |= !(fabsf(off) <= 0.49975586f);  // 0.5 - 2^-12; NaN and infinity too
-    const int c = static_cast<int>(__float_as_uint(t)) - static_cast<int>(__float_as_uint(magic));
-    word |= static_cast<uint32_t>(min(max(c, 0), 15)) << (4 * i);
+    int32_t bits = __float_as_int(t);  // magic's bits plus the code
+    // not within 0.5 - 2^-16 of the integer (four times what 15 2^-22 is off), or NaN
+    if (!(fabsf(__fmaf_rn(d, inv, -__fsub_rn(t, magic))) <= 0.49998474f))
+      bits = __float_as_int(magic + fminf(fmaxf(rintf(__fdiv_rn(d, s)), 0.f), 15.f));
+    if (!kExact) bits = min(max(bits, __float_as_int(magic)), __float_as_int(magic) + 15);
+    word = word * 16u + static_cast<uint32_t>(bits);
   }
-  if (near) {
-    word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fdiv_rn(__fsub_rn(x[i], m), s));
-      word |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
-    }
-  }
-  return word;
+  return word - 0x3f400000u;         // the sum of magic's bits (0x4b400000) 16^i, modulo 2^32
 }
 
 constexpr int kTokensPerCta = kRowsPerCta / 2;  // K and V
@@ -93,47 +116,60 @@ __global__ void __launch_bounds__(kThreads)
                           uint8_t *__restrict__ k_cache, uint8_t *__restrict__ v_cache,
                           int64_t k_block_stride, int64_t v_block_stride,
                           const int32_t *__restrict__ slots, int32_t tokens, int32_t hkv,
-                          int32_t block_size, int32_t num_blocks, uint32_t *err) {
-  const int lane = threadIdx.x & 31, sub = lane & 15;
-  // a warp holds K and V of one token: every lane takes part in the shuffles
-  const bool is_v = lane >= 16;
-  const int32_t chunk = blockIdx.x / hkv, h = blockIdx.x - chunk * hkv;
-  const int32_t t = chunk * kTokensPerCta + (threadIdx.x >> 5);
-  if (t >= tokens) return;
-  const int32_t slot = __ldg(slots + t);
-  const int32_t blk = slot / block_size, off = slot - blk * block_size;
-  if (slot < 0 || blk >= num_blocks) {
-    if (slot != -1 && lane == 0) record_error(err, SLOKV_DEVERR_SLOT_RANGE);
-    return;
-  }
-  float x[8];
-  const T *src = is_v ? value + t * value_stride + h * value_head : key + t * key_stride + h * key_head;
-  load8<T, kVec>(src + sub * 8, x);
-  float mn = x[0], mx = x[0];
-  bool bad = false;
+                          int32_t block_size, int32_t num_blocks, FastDiv by_hkv, FastDiv by_block,
+                          uint32_t *err) {
+  const int lane = threadIdx.x & 31, sub = lane & 7;
+  // a warp holds K and V of two tokens; every lane takes part in the shuffles
+  const bool is_v = lane & 8;
+  const int32_t chunk = by_hkv(blockIdx.x), h = blockIdx.x - chunk * hkv;
+  const int32_t t = chunk * kTokensPerCta + (threadIdx.x >> 4);
+  const int32_t slot = t < tokens ? __ldg(slots + t) : -1;
+  const int32_t blk = by_block(max(slot, 0)), off = slot - blk * block_size;
+  const bool live = slot >= 0 && blk < num_blocks;
+  if (!live && slot != -1 && sub == 0) record_error(err, SLOKV_DEVERR_SLOT_RANGE);
+  float x[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 16; ++i) x[i] = 0.f;
+  if (live) {
+    const T *src = (is_v ? value + t * value_stride + h * value_head : key + t * key_stride + h * key_head) +
+                   sub * 16;
+    load8<T, kVec>(src, x);
+    load8<T, kVec>(src + 8, x + 8);
+  }
+  float mn = x[0], mx = x[0], zero = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
     mn = fminf(mn, x[i]);
     mx = fmaxf(mx, x[i]);
-    bad |= !isfinite(x[i]);
+    zero = __fmaf_rn(x[i], 0.f, zero);  // NaN where a value is not finite
   }
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
+  for (int o = 1; o < 4; o <<= 1) {
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
-  const uint32_t votes = __ballot_sync(0xffffffffu, bad);
-  bad = (votes >> (lane & 24)) & 0xffu;
+  const uint32_t votes = __ballot_sync(0xffffffffu, zero != zero);
+  bool bad = (votes >> (lane & 28)) & 0xfu;
   const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(mx, mn), 15.f));
   const __nv_bfloat16 mb = __float2bfloat16_rn(mn);
   const float s = __bfloat162float(sb), m = __bfloat162float(mb);
   bad |= !isfinite(s) || !isfinite(m);
-  const uint32_t word = !bad && s > 0.f ? encode8(x, m, s) : 0u;
+  uint32_t w0 = 0, w1 = 0;
+  if (!bad && s > 0.f) {
+    constexpr bool kExact = std::is_same<T, __nv_bfloat16>::value;  // other minima may round up
+    const float inv = s < 7.5e-37f ? __int_as_float(0x7fffffff) : rcp_fast(s);
+    w0 = encode8<kExact>(x, m, s, inv);
+    w1 = encode8<kExact>(x + 8, m, s, inv);
+  }
+  // lane j of group 0 has the row's stored words 4j, 4j + 2 and lane j of group 1 4j + 1, 4j + 3
+  const int grp = sub >> 2, j = sub & 3;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, grp ? w0 : w1, 4);
+  if (!live) return;
   uint8_t *run = (is_v ? v_cache + blk * v_block_stride : k_cache + blk * k_block_stride) +
                  static_cast<int64_t>(h) * block_size * kRowBytes;
-  const int grp = sub >> 3, i = sub & 7;
-  *reinterpret_cast<uint32_t *>(run + code_offset(off) + (2 * i + grp) * 4) = word;
-  if (i == 0) {
+  *reinterpret_cast<uint2 *>(run + code_offset(off) + 16 * j + 8 * grp) =
+      grp ? make_uint2(other, w1) : make_uint2(w0, other);
+  if (j == 0) {
     const uint32_t lo = bad ? 0x7fffu : __bfloat16_as_ushort(sb);
     const uint32_t hi = bad ? 0u : __bfloat16_as_ushort(mb);
     *reinterpret_cast<uint32_t *>(run + param_offset(off) + 4 * grp) = lo | (hi << 16);
@@ -323,7 +359,8 @@ extern "C" int slokv_kv_append_int4(const void *key, int64_t key_row_stride,
         static_cast<const T *>(key), key_row_stride, key_head_stride,
         static_cast<const T *>(value), value_row_stride, value_head_stride,
         static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_block_stride,
-        v_block_stride, slot_mapping, num_tokens, num_kv_heads, block_size, num_blocks, dev_error);
+        v_block_stride, slot_mapping, num_tokens, num_kv_heads, block_size, num_blocks,
+        FastDiv(num_kv_heads), FastDiv(block_size), dev_error);
     return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
   };
   if (in_dtype == SLOKV_DTYPE_BF16)
