@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictPa
   __shared__ uint32_t hist[kCopies][256];
   __shared__ uint32_t sh_prefix, sh_left, sh_done;
   __shared__ uint32_t piece[3][kWarps];   // ties, holes, moved tokens of each warp's piece
+  launch_dependents();  // the move kernel
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv;
   const int32_t n = __ldg(p.lens + b);
@@ -247,6 +248,7 @@ __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictPa
 
 __global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const EvictParams p) {
   const int32_t pair = blockIdx.x, b = pair / p.hkv, h = pair % p.hkv;
+  wait_prerequisites();
   const int32_t count = __ldg(p.counts + pair);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int32_t *dst = p.moves + static_cast<int64_t>(pair) * 2 * p.max_moves;
@@ -412,6 +414,7 @@ extern "C" int slokv_kv_evict(void *k_cache, void *v_cache, int64_t k_block_stri
   if (cudaGetLastError() != cudaSuccess) return SLOKV_ERR_CUDA;
   if (most == 0) return SLOKV_OK;
   const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(chunks));
-  kv_evict_move_kernel<<<grid, kMoveThreads, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
+  return launch_dependent(kv_evict_move_kernel, grid, dim3(kMoveThreads), 0, st, p) == cudaSuccess
+             ? SLOKV_OK
+             : SLOKV_ERR_CUDA;
 }

@@ -41,6 +41,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 template <bool kPairs, bool kVec>
 __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const ScoreParams p) {
   const int32_t b = blockIdx.z, h = blockIdx.y;
+  wait_prerequisites();
   int32_t len = __ldg(p.lens + b);
   const int32_t row = p.rows ? __ldg(p.rows + b) : b;
   const bool first = blockIdx.x == 0 && h == 0 && threadIdx.x == 0;
@@ -166,10 +167,9 @@ extern "C" int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int
                   static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (logits_pairs && (reinterpret_cast<uintptr_t>(logits) & 7u)) return SLOKV_ERR_ALIGNMENT;
-  auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, st>>>(p); };
-  if (logits_pairs)
-    go(kv_scores_accumulate_kernel<true, false>);
-  else
-    vec ? go(kv_scores_accumulate_kernel<false, true>) : go(kv_scores_accumulate_kernel<false, false>);
-  return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
+  auto *kernel = logits_pairs ? kv_scores_accumulate_kernel<true, false>
+                 : vec        ? kv_scores_accumulate_kernel<false, true>
+                              : kv_scores_accumulate_kernel<false, false>;
+  return launch_dependent(kernel, grid, dim3(kThreads), 0, st, p) == cudaSuccess ? SLOKV_OK
+                                                                                : SLOKV_ERR_CUDA;
 }

@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
 
+  if constexpr (kScored) launch_dependents();  // the merge kernel
   if (threadIdx.x == 0) {
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
@@ -656,6 +657,10 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
 // independent loads; lane l owns dims [4l, 4l+4).
 template <typename T, bool kScored = false>
 __global__ void __launch_bounds__(128) paged_decode_merge_kernel(const Params p) {
+  if constexpr (kScored) {
+    launch_dependents();  // the accumulation of the scores
+    wait_prerequisites();
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t s = blockIdx.x;
   if (s >= p.nslots) return;
@@ -791,6 +796,11 @@ int launch(const Params &p0, const CUtensorMap &km, const CUtensorMap &vm, int s
   if (!ok) return SLOKV_ERR_CUDA;
   paged_decode_kernel<T, kFp8, kScored><<<sms, kW * 32, smem, stream>>>(km, vm, p0);
   if (cudaGetLastError() != cudaSuccess) return SLOKV_ERR_CUDA;
+  if (kScored)
+    return launch_dependent(paged_decode_merge_kernel<T, kScored>, dim3(p0.nslots), dim3(128), 0, stream,
+                            p0) == cudaSuccess
+               ? SLOKV_OK
+               : SLOKV_ERR_CUDA;
   paged_decode_merge_kernel<T, kScored><<<p0.nslots, 128, 0, stream>>>(p0);
   return cudaGetLastError() == cudaSuccess ? SLOKV_OK : SLOKV_ERR_CUDA;
 }

@@ -348,8 +348,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
   const uint32_t bars_all = base + kRingBytes;
   int32_t *prefix = reinterpret_cast<int32_t *>(base_ptr + kRingBytes + kWarps * kStages * 8);
 
-  // the merge kernel may be set up while this one runs; it waits for its completion
-  asm volatile("griddepcontrol.launch_dependents;");
+  launch_dependents();  // the merge kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
 
@@ -800,7 +799,7 @@ __device__ __forceinline__ void merge_into(Merged &x, const Merged &y) {
 template <typename T, bool kScored>
 __global__ void __launch_bounds__(kMergeThreads) paged_decode_int4_merge_kernel(const Params p) {
   __shared__ Merged part[kMergeGroups][8];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_prerequisites();
   const int32_t s = blockIdx.x;
   const int4 job = p.jobs[s];
   if (job.x < 0) return;
@@ -896,17 +895,9 @@ int launch(const Params &p, int dev, int sms, cudaStream_t stream) {
   paged_decode_int4_kernel<T, kN, kScored><<<sms, kWarps * 32, smem_bytes(kWarps, p.batch),
                                             stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SLOKV_ERR_CUDA;
-  // set up while the main kernel runs; griddepcontrol.wait holds it until that is done
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.nslots));
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_decode_int4_merge_kernel<T, kScored>, p) == cudaSuccess
+  return launch_dependent(paged_decode_int4_merge_kernel<T, kScored>,
+                          dim3(static_cast<unsigned>(p.nslots)), dim3(kMergeThreads), 0, stream,
+                          p) == cudaSuccess
              ? SLOKV_OK
              : SLOKV_ERR_CUDA;
 }
