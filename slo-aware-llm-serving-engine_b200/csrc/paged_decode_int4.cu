@@ -21,16 +21,15 @@
 // columns of both products, so no MMA row is wasted on a small group, and a lane's
 // score and output columns are the same two heads.  movmatrix turns the score tile into
 // the B operand; a prmt pairs the codes of two tokens, then the same masks apply.  The
-// probabilities carry the V scale, r = f16(p s_g) (half a step is 2^-11, an eighth of
-// a bf16 output's), out = sum_t r c + sum_t p m.  For f16 outputs, which round as finely
-// as r does,
-//   out = sum_t r (c - 8) + sum_t p (m + 8 s)
-// with sum_t 8 r from one more MMA with a constant A, so that the rounding of r meets
-// c - 8 instead of c: 3.3e-4 instead of 5e-4 off in all, for 2 % of the time.  f16 has 5
-// exponent bits and the scales' range is fp32's: the reference that the scores are exponentiated against is not the running maximum
-// but lies 15 - ceil(log2 max(s, |m|)) below it, the maximum over the tokens seen so
-// far.  r is then at most 2^15 and keeps its 11 bits down to 2^-29 of the largest value;
-// the sum of p is taken against the same reference, so the quotient does not see it.
+// probabilities carry the V scale, r = f16(p s_g):  out = sum_t r c + sum_t p m.  Half a step
+// of r is 2^-11, an eighth of a bf16 output's (1.8e-3 off in all, 1.7e-3 of it the
+// output's).  An f16 output rounds as finely as r does, so for those r is two f16 (the second
+// takes what the first leaves) and the product runs twice: 2.1e-4 off, the output's own,
+// instead of 5e-4 with one.  f16 has 5 exponent bits and the scales' range is fp32's: the
+// reference that the scores are exponentiated against is not the running maximum but lies
+// 15 - ceil(log2 max(s, |m|)) below it, the maximum over the tokens seen so far.  r is then
+// at most 2^15 and keeps its 11 bits down to 2^-29 of the largest value; the sum of p is
+// taken against the same reference, so the quotient does not see it.
 //
 // Work split: the 64-token tiles of all (sequence, kv head) segments, in that order, cut
 // into equal contiguous ranges, one per warp slot; slot s is warp s / grid of CTA s % grid,
@@ -341,7 +340,7 @@ template <typename T, int kN, bool kScored>
 __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel(const Params p) {
   using MO = Mma<T>;
   constexpr int kWarps = warps_of(kN), kRingBytes = ring_bytes(kWarps);
-  constexpr bool kCentre = std::is_same<T, __half>::value;
+  constexpr int kParts = std::is_same<T, __half>::value ? 2 : 1;  // f16 pieces of p s
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
   uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -481,10 +480,9 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
     }
 
     // out^T accumulators: o[rr][4 grp + k][x] is dim 64 grp + 8 g + k (+ 4 for x >= 2) of head
-    // 8 rr + 2 c + (x & 1), 16 times larger for odd k; osum: 8 sum r of the same heads;
-    // vz: sum of p (m + 8 s) over this lane's tokens.  m: running maximum score, ref: what
-    // the scores are exponentiated against.
-    float o[kN][8][4], osum[kN][2][4], vz[kN][2][2], m[kN][2], ref[kN][2], l[kN][2];
+    // 8 rr + 2 c + (x & 1), 16 times larger for odd k; vz: sum of p m over this lane's
+    // tokens.  m: running maximum score, ref: what the scores are exponentiated against.
+    float o[kN][8][4], vz[kN][2][2], m[kN][2], ref[kN][2], l[kN][2];
     int sexp = -100;  // ceil(log2) of the largest V scale or minimum so far
 #pragma unroll
     for (int rr = 0; rr < kN; ++rr) {
@@ -492,7 +490,6 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
       for (int n = 0; n < 8; ++n) o[rr][n][0] = o[rr][n][1] = o[rr][n][2] = o[rr][n][3] = 0.f;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        osum[rr][n][0] = osum[rr][n][1] = osum[rr][n][2] = osum[rr][n][3] = 0.f;
         vz[rr][n][0] = vz[rr][n][1] = 0.f;
         m[rr][n] = ref[rr][n] = -INFINITY;
         l[rr][n] = 0.f;
@@ -646,8 +643,6 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
           }
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            osum[rr][n][0] *= alpha[rr][0];
-            osum[rr][n][1] *= alpha[rr][1];
             vz[rr][n][0] *= alpha[rr][0];
             vz[rr][n][1] *= alpha[rr][1];
             l[rr][n] *= alpha[rr][n];
@@ -658,13 +653,11 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
       // ---- out^T += V^T P^T, 16 tokens a step ----
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t pb[kN][2][2];  // [head columns][group][b0 | b1]
+        uint32_t pb[kParts][kN][2][2];  // [piece][head columns][group][b0 | b1]
 #pragma unroll
         for (int row = 0; row < 2; ++row) {
           const uint2 pw = lds64(vb + kParamOff + (16 * i + 8 * row + tok_k) * 8);
-          const float s0 = scale_of(pw.x), s1 = scale_of(pw.y);
-          const float z0 = kCentre ? fmaf(8.f, s0, min_of(pw.x)) : min_of(pw.x);
-          const float z1 = kCentre ? fmaf(8.f, s1, min_of(pw.y)) : min_of(pw.y);
+          const float s0 = scale_of(pw.x), s1 = scale_of(pw.y), m0 = min_of(pw.x), m1 = min_of(pw.y);
 #pragma unroll
           for (int rr = 0; rr < kN; ++rr) {
             float pr[2];
@@ -672,11 +665,20 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
             for (int x = 0; x < 2; ++x) {
               pr[x] = fast_exp2(fmaf(sc[rr][i][2 * row + x], unscale[rr][x], -ref[rr][x]));
               l[rr][x] += pr[x];
-              vz[rr][0][x] = fmaf(pr[x], z0, vz[rr][0][x]);
-              vz[rr][1][x] = fmaf(pr[x], z1, vz[rr][1][x]);
+              vz[rr][0][x] = fmaf(pr[x], m0, vz[rr][0][x]);
+              vz[rr][1][x] = fmaf(pr[x], m1, vz[rr][1][x]);
             }
-            pb[rr][0][row] = movmatrix_trans(Mma<__half>::pack(pr[0] * s0, pr[1] * s0));
-            pb[rr][1][row] = movmatrix_trans(Mma<__half>::pack(pr[0] * s1, pr[1] * s1));
+            const uint32_t r0 = Mma<__half>::pack(pr[0] * s0, pr[1] * s0);
+            const uint32_t r1 = Mma<__half>::pack(pr[0] * s1, pr[1] * s1);
+            pb[0][rr][0][row] = movmatrix_trans(r0);
+            pb[0][rr][1][row] = movmatrix_trans(r1);
+            if constexpr (kParts == 2) {
+              const float2 f0 = Mma<__half>::unpack(r0), f1 = Mma<__half>::unpack(r1);
+              pb[1][rr][0][row] = movmatrix_trans(
+                  Mma<__half>::pack(fmaf(pr[0], s0, -f0.x), fmaf(pr[1], s0, -f0.y)));
+              pb[1][rr][1][row] = movmatrix_trans(
+                  Mma<__half>::pack(fmaf(pr[0], s1, -f1.x), fmaf(pr[1], s1, -f1.y)));
+            }
           }
         }
         const uint2 e0 = lds64(vb + (16 * i + tok_e) * 64 + g * 8);
@@ -695,13 +697,12 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
             const int sh = k & 2 ? 8 : 0;
 #pragma unroll
             for (int rr = 0; rr < kN; ++rr)
-              mma_f16(o[rr][4 * grp + k], (lo0 >> sh) & mask, (hi0 >> sh) & mask,
-                      (lo1 >> sh) & mask, (hi1 >> sh) & mask, pb[rr][grp][0], pb[rr][grp][1]);
-          }
 #pragma unroll
-          for (int rr = 0; kCentre && rr < kN; ++rr)
-            mma_f16(osum[rr][grp], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u,
-                    pb[rr][grp][0], pb[rr][grp][1]);
+              for (int part = 0; part < kParts; ++part)
+                mma_f16(o[rr][4 * grp + k], (lo0 >> sh) & mask, (hi0 >> sh) & mask,
+                        (lo1 >> sh) & mask, (hi1 >> sh) & mask, pb[part][rr][grp][0],
+                        pb[part][rr][grp][1]);
+          }
         }
       }
       __syncwarp();
@@ -744,7 +745,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
           // 2^24 undoes the codes' unit, 2^20 that of the codes 16 times larger
-          const float z = kCentre ? fmaf(-16777216.f, osum[rr][grp][x], vz[rr][grp][x]) : vz[rr][grp][x];
+          const float z = vz[rr][grp][x];
           float v[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {

@@ -3,16 +3,17 @@ restatements (tests/int4_reference.py).
 
 Tolerances.  Stored bytes are compared exactly.  Decode (derived from the kernel's
 arithmetic, u = 2^-24, half a step of fp32):
-  * the rounding of p s to f16 meets c s (bf16 outputs) or (c - 8) s (f16 outputs):
-    2^-11 sum_t w_t s_t c_t, or |c_t - 8| (plus nothing below 2^-29 of the largest scale,
-    which the cases do not reach);
+  * p s is rounded to f16, to two f16 for f16 outputs: 2^-11 or 2^-22 of sum_t w_t s_t c_t
+    (plus nothing below 2^-29 of the largest value, which the cases do not reach; the second
+    f16's own smallest step is 2^-25 against a largest p s of 2^14 at least, so another
+    2^-38 of the largest value a token);
   * an error e in a score changes its weight by a factor within 1 +- 2 e: e <= (128 + 16)
     products and sums in fp32, each within u of their absolute sum, so e <= 400 u
     scale sum_d |q_d| (15 s + |m|) with the tensor core's truncation counted double;
     the exponential adds 2^-21;  out moves by at most (2 e + 2^-20) sum_t w_t |v_t|;
-  * accumulating sum r c and 8 sum r over n tokens: one rounding (2 u) per MMA and per
-    tile of the running sums, which are at most 15 and 8 times sum w s:
-    (n / 16 + 40) 2 u 32 sum_t w_t s_t, and (n / 2 + 40) 2 u for sum p (m + 8 s);
+  * accumulating sum r c over n tokens: one rounding (2 u) per MMA and per
+    tile of the running sum, which is at most 15 sum w s:
+    (n / 16 + 40) 2 u 32 sum_t w_t s_t, and (n / 2 + 40) 2 u for sum p |m|;
   * the output's own rounding: 2^-8 (bf16) or 2^-11 (f16) of the value, and f16's
     smallest step 2^-25.
 """
@@ -62,14 +63,18 @@ def decode_bound(q, k, v, ks, vs, kmin_abs, w, out, scale, dtype):
     rep = lambda x: x.repeat_interleave(G, 1)
     s_dim = rep(vs).repeat_interleave(64, -1)                       # [n, Hq, 128]
     vv = rep(v)
-    middle = 8 if dtype == torch.float16 else 0
-    centre = (vv - (rep(kmin_abs[1]).repeat_interleave(64, -1) + middle * s_dim)).abs()
+    vmin = rep(kmin_abs[1]).repeat_interleave(64, -1)
+    above = (vv - vmin).abs()                                       # s c
     k_abs = rep(kmin_abs[0].abs() + 15 * ks).repeat_interleave(64, -1)
     e = 400 * U * abs(scale) * torch.einsum("hd,nhd->hn", q.double().abs(), k_abs).max(-1).values
     wv = torch.einsum("hn,nhd->hd", w, vv.abs())
     ws = torch.einsum("hn,nhd->hd", w, s_dim)
-    wz = torch.einsum("hn,nhd->hd", w, (rep(kmin_abs[1]).repeat_interleave(64, -1) + 8 * s_dim).abs())
-    b = 2.0 ** -11 * torch.einsum("hn,nhd->hd", w, centre)
+    wz = torch.einsum("hn,nhd->hd", w, vmin.abs())
+    wc = torch.einsum("hn,nhd->hd", w, above)
+    if dtype == torch.float16:
+        b = 2.0 ** -22 * wc + n * 2.0 ** -38 * 15 * torch.maximum(s_dim, vmin.abs()).amax((0, 2)).unsqueeze(-1)
+    else:
+        b = 2.0 ** -11 * wc
     b = b + (2 * e + 2.0 ** -20).unsqueeze(-1) * wv
     b = b + (n / 16 + 40) * 2 * U * 32 * ws + (n / 2 + 40) * 2 * U * wz
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
