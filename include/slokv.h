@@ -436,8 +436,8 @@ int slokv_int4_decode(const void *cache, int64_t block_stride, const int32_t *sl
  * pages_per_row]) is filled with those page ids, ready for slokv_paged_prefill
  * (block_size 128).  Values are rounded once to dst_dtype.  Pages that a row reaches
  * are written whole (zeros past its keys), the others not at all.  A block id
- * outside the pool reads as zeros and sets SLOKV_DEVERR_BLOCK_RANGE; keys past the
- * table's reach set SLOKV_DEVERR_CONTEXT_LEN. */
+ * outside the pool reads as zeros and sets SLOKV_DEVERR_BLOCK_RANGE; so do keys past
+ * the table's reach, with SLOKV_DEVERR_CONTEXT_LEN. */
 int slokv_int4_rows_widen(const void *k_cache, const void *v_cache, int64_t k_block_stride,
                           int64_t v_block_stride, int32_t num_blocks, int32_t block_size,
                           int32_t num_kv_heads, int32_t head_dim, const int32_t *block_tables,

@@ -246,13 +246,13 @@ __global__ void __launch_bounds__(kThreads)
   const bool first = h == 0 && !is_v && threadIdx.x == 0;
   if (first) dst_table[blockIdx.x] = blockIdx.x;
   int64_t keys = static_cast<int64_t>(__ldg(cu_k + r + 1)) - __ldg(cu_k + r);
+  const int64_t t0 = static_cast<int64_t>(page) * kWidePage;
+  if (t0 >= keys) return;
   const int64_t reach = static_cast<int64_t>(max_blocks) * block_size;
-  if (keys > reach) {
+  if (keys > reach) {                             // keys past the table read as zeros
     if (first && page == 0) record_error(err, SLOKV_DEVERR_CONTEXT_LEN);
     keys = reach;
   }
-  const int64_t t0 = static_cast<int64_t>(page) * kWidePage;
-  if (t0 >= keys) return;
   const uint8_t *cache = is_v ? v_cache : k_cache;
   const int64_t stride = is_v ? v_block_stride : k_block_stride;
   T *dst = (is_v ? dst_v : dst_k) +

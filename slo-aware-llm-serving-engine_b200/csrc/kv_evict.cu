@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictPa
 __global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const EvictParams p) {
   const int32_t pair = blockIdx.x, b = pair / p.hkv, h = pair % p.hkv;
   wait_prerequisites();
-  const int32_t count = __ldg(p.counts + pair);
+  // (the selection's output: through L2, since this kernel may have started before it)
+  const int32_t count = __ldcg(p.counts + pair);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int32_t *dst = p.moves + static_cast<int64_t>(pair) * 2 * p.max_moves;
   const int32_t *src = dst + p.max_moves;
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const Evict
   if (first >= count) return;
   int32_t tb = -1, fb = 0, to_off = 0, from_off = 0;
   if (lane < kMovesPerWarp && first + lane < count) {
-    const int32_t to = __ldg(dst + first + lane), from = __ldg(src + first + lane);
+    const int32_t to = __ldcg(dst + first + lane), from = __ldcg(src + first + lane);
     const int32_t to_page = to / p.block_size, from_page = from / p.block_size;
     tb = __ldg(table + to_page);
     fb = __ldg(table + from_page);

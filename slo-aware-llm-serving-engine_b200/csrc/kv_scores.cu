@@ -7,7 +7,9 @@
 // read a second time).  One thread takes four tokens of one head and adds its group
 // in order: no atomics, the same sum on every run.  The bf16 / f16 decode stores a row of
 // tokens per head, the 4-bit decode the heads of a token side by side (what their
-// accumulators make contiguous); both are read here.
+// accumulators make contiguous); both are read here.  The kernel may start before those
+// that store them have ended, so what they store is loaded through L2 (__ldcg) and not
+// through the read-only path.
 #include "common.cuh"
 
 namespace slokv {
@@ -72,11 +74,11 @@ __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const Sc
 #pragma unroll 2
     for (int g = 0; g < p.group; g += 2) {
       // a head whose every score is -inf has no weights; nor has the padding
-      const float d0 = __ldg(lse + g), d1 = g + 1 < p.group ? __ldg(lse + g + 1) : -INFINITY;
+      const float d0 = __ldcg(lse + g), d1 = g + 1 < p.group ? __ldcg(lse + g + 1) : -INFINITY;
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (t0 + i * kThreads < len) {
-          const float2 x = __ldg(reinterpret_cast<const float2 *>(lg + i * step + g));
+          const float2 x = __ldcg(reinterpret_cast<const float2 *>(lg + i * step + g));
           if (d0 != -INFINITY) w[i] += exp2_fast(x.x - d0);
           if (d1 != -INFINITY) w[i] += exp2_fast(x.y - d1);
         }
@@ -95,15 +97,15 @@ __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const Sc
     if (kVec && n == kPer && p.decay != 0.f) before = *reinterpret_cast<const float4 *>(score + t);
 #pragma unroll 4
     for (int g = 0; g < p.group; ++g, lg += p.logits_stride) {
-      const float d = __ldg(lse + g);
+      const float d = __ldcg(lse + g);
       if (d == -INFINITY) continue;
       float x[kPer];
       if (kVec && n == kPer) {
-        const float4 v = __ldg(reinterpret_cast<const float4 *>(lg));
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(lg));
         x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
       } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] = i < n ? __ldg(lg + i) : 0.f;
+        for (int i = 0; i < kPer; ++i) x[i] = i < n ? __ldcg(lg + i) : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < kPer; ++i) w[i] += exp2_fast(x[i] - d);

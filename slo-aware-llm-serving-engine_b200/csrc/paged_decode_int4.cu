@@ -28,8 +28,9 @@
 // instead of 5e-4 with one.  f16 has 5 exponent bits and the scales' range is fp32's: the
 // reference that the scores are exponentiated against is not the running maximum but lies
 // 15 - ceil(log2 max(s, |m|)) below it, the maximum over the tokens seen so far.  r is then
-// at most 2^15 and keeps its 11 bits down to 2^-29 of the largest value; the sum of p is
-// taken against the same reference, so the quotient does not see it.
+// at most 2^15 and keeps its 11 bits down to 2^-29 of the largest value (or of 2^-60, if
+// that is more); the sum of p is taken against the same reference, so the quotient does not
+// see it.
 //
 // Work split: the 64-token tiles of all (sequence, kv head) segments, in that order, cut
 // into equal contiguous ranges, one per warp slot; slot s is warp s / grid of CTA s % grid,
@@ -483,7 +484,9 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
     // 8 rr + 2 c + (x & 1), 16 times larger for odd k; vz: sum of p m over this lane's
     // tokens.  m: running maximum score, ref: what the scores are exponentiated against.
     float o[kN][8][4], vz[kN][2][2], m[kN][2], ref[kN][2], l[kN][2];
-    int sexp = -100;  // ceil(log2) of the largest V scale or minimum so far
+    // ceil(log2) of the largest V scale or minimum so far; at least -60, so that the sum of
+    // p <= 2^75 stays finite over any context (V values all zero)
+    int sexp = -60;
 #pragma unroll
     for (int rr = 0; rr < kN; ++rr) {
 #pragma unroll
@@ -606,8 +609,10 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
           const uint32_t w[4] = {p0.x & abs2, p0.y & abs2, p1.x & abs2, p1.y & abs2};
           top = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if ((w[i] & 0xffffu) < 0x7f80u) top = max(top, max(w[i] >> 16, w[i] & 0xffffu));
+          for (int i = 0; i < 4; ++i) {
+            if ((w[i] & 0xffffu) < 0x7f80u) top = max(top, w[i] & 0xffffu);
+            if ((w[i] >> 16) < 0x7f80u) top = max(top, w[i] >> 16);
+          }
           top = __reduce_max_sync(0xffffffffu, top);
         }
         sexp = max(sexp, static_cast<int>(top >> 7) - 126);

@@ -161,8 +161,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     shared ones first); those past it can be freed afterwards.
     """
     keep, recent = int(keep), int(recent)
-    if keep < 1 or recent < 0 or recent > keep:
-        raise SlokvError("kv_evict needs keep >= 1 and 0 <= recent <= keep")
+    if not 1 <= keep < 2 ** 31 or not 0 <= recent <= keep:
+        raise SlokvError("kv_evict needs 1 <= keep < 2^31 and 0 <= recent <= keep")
     if is_int4_cache(k_cache):
         NB, bs, Hkv, k_block, v_block = int4_geometry(k_cache, v_cache)
         dtype = _lib.DTYPE_INT4

@@ -31,7 +31,7 @@ _WIDE_PAGE = 128        # tokens of a page that rows are widened to for prefill
 # on L 4000 82 / 63, of 128 79 / 110; 8 rows of 16 115 / 109, of 32 113 / 202; 64 rows
 # of 4 793 / 204, of 16 783 / 783).
 SHORT_CHUNK, SHORT_CALL = 16, 64
-_MAX_DECODE_ROWS = 8192
+_MAX_DECODE_ROWS, _MAX_GROUP = 8192, 16   # of the decode kernel
 
 _Q_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _STORE_DTYPES = {**_Q_DTYPES, torch.float32: _lib.DTYPE_F32}
@@ -243,10 +243,13 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != q.shape or out.stride(-1) != 1:
         raise SlokvError("out must match q's shape and dtype with a contiguous last dim")
-    if Tq == 0 or rows <= 0 or int(max_seqlen_q) <= 0:
+    max_seqlen_q, max_seqlen_k = int(max_seqlen_q), int(max_seqlen_k)
+    if Tq == 0 or rows <= 0 or max_seqlen_q <= 0:
         return out
+    if block_table.shape[1] == 0:
+        raise SlokvError("block_table has no columns")
     if ((max_seqlen_q <= SHORT_CHUNK or Tq <= SHORT_CALL) and Tq <= _MAX_DECODE_ROWS
-            and block_table.shape[1]):
+            and Hq // Hkv <= _MAX_GROUP):
         scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
         with on_device(dev) as stream:
             nbytes = decode_int4_workspace_bytes(dev.index, Hq, Hkv)
@@ -259,7 +262,7 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
                                ws.data_ptr(), nbytes, buffers.error_word(dev).data_ptr(), stream,
                                table_rows=table_rows)
         return out
-    pages = max(1, (int(max_seqlen_k) + _WIDE_PAGE - 1) // _WIDE_PAGE)
+    pages = max(1, (max_seqlen_k + _WIDE_PAGE - 1) // _WIDE_PAGE)
     with on_device(dev) as stream:
         wide = torch.empty(2, rows * pages, _WIDE_PAGE, Hkv, HEAD_DIM, dtype=q.dtype, device=dev)
         table = torch.empty(rows, pages, dtype=torch.int32, device=dev)

@@ -332,6 +332,25 @@ def test_decode_value_range(pkg):
         check_decode(out, q[i:i + 1], kp, vp, [n], tables[:1], scale)
 
 
+def test_decode_values_all_zero(pkg):
+    """Thousands of tokens whose V rows are all zero (the reference that the scores are taken
+    against then lies far above the others'), alone and before rows that are not."""
+    bs, n = 256, 9000
+    nb = (n + bs - 1) // bs
+    kp = make_pool(pkg, 65, nb, bs, 1)
+    vp = torch.zeros_like(kp)
+    tables = torch.arange(nb, dtype=torch.int32).view(1, -1)
+    q = torch.from_numpy(det_normal(66, (1, 1, 2, 128))).float().bfloat16()
+    ln = torch.tensor([n], dtype=torch.int32).cuda()
+    scores = torch.zeros(1, 1, n, device="cuda")
+    out = pkg.flash_attn_with_kvcache_scored(q.cuda(), kp, vp, scores, ln, tables.cuda())
+    assert (out == 0).all() and abs(scores.sum().item() - 2) < 2 * 2.0 ** -16
+    one = make_pool(pkg, 67, 1, bs, 1)
+    vp[nb - 1] = one[0]
+    out = pkg.flash_attn_with_kvcache_int4(q.cuda(), kp, vp, ln, tables.cuda())
+    check_decode(out, q, kp, vp, [n], tables, 128 ** -0.5)
+
+
 def test_decode_nan_stays_in_its_group(pkg):
     n, bs = 70, 128
     k = torch.from_numpy(det_normal(71, (n, 1, 128))).float().bfloat16()
@@ -393,6 +412,7 @@ def test_decode_captured_twice_and_other_stream(pkg):
     ([7, 0, 12], [9, 100, 500], 1, 1, 64, torch.float16),
     ([16] * 5, [0, 0, 300, 63, 64], 2, 8, 64, torch.bfloat16),
     ([17] * 5, [0, 0, 300, 63, 64], 2, 8, 64, torch.bfloat16),
+    ([4], [200], 1, 24, 64, torch.bfloat16),            # a wider group than the decode takes
 ])
 def test_varlen(pkg, qlens, hist, H, G, bs, dtype):
     """Short calls (SHORT_CHUNK, SHORT_CALL) run as decode rows and have their bound.  Longer
@@ -423,7 +443,7 @@ def test_varlen(pkg, qlens, hist, H, G, bs, dtype):
     assert pkg.read_device_errors() == 0
     from importlib import import_module
     K = import_module("slo-aware-llm-serving-engine_b200.kvcache_int4")
-    if max(qlens) <= K.SHORT_CHUNK or sum(qlens) <= K.SHORT_CALL:
+    if (max(qlens) <= K.SHORT_CHUNK or sum(qlens) <= K.SHORT_CALL) and G <= 16:
         seen = [nk - nq + i + 1 for nq, nk in zip(qlens, klens) for i in range(nq)]
         per = torch.cat([tables[b:b + 1].expand(nq, -1) for b, nq in enumerate(qlens)])
         check_decode(out.unsqueeze(1), q.unsqueeze(1), kp, vp, seen, per, 128 ** -0.5)
@@ -452,9 +472,11 @@ def test_varlen_bad_metadata_is_flagged(pkg, nq):
     out = pkg.flash_attn_varlen_func_int4(q, kp, vp, cu_q, cu_k, nq, 100, block_table=torch.tensor(
         [[1, 9]], dtype=torch.int32, device="cuda"))
     assert pkg.read_device_errors() & 0x2 and torch.isfinite(out).all()
-    pkg.flash_attn_varlen_func_int4(q, kp, vp, cu_q, cu_k, nq, 100, block_table=torch.tensor(
+    # more keys than the table reaches, by more than one widened page
+    cu_k = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    out = pkg.flash_attn_varlen_func_int4(q, kp, vp, cu_q, cu_k, nq, 300, block_table=torch.tensor(
         [[1]], dtype=torch.int32, device="cuda"))
-    assert pkg.read_device_errors() & 0x4
+    assert pkg.read_device_errors() & 0x4 and torch.isfinite(out).all()
 
 
 @pytest.mark.parametrize("nq", [3, 66])

@@ -131,6 +131,6 @@ def test_python_refusals(pkg):
         pkg.flash_attn_with_kvcache_scored(q, fp8, fp8, torch.zeros(2, 2, 8), ln, bt)
     with pytest.raises(E):
         pkg.kv_evict(fp8, fp8, torch.zeros(2, 2, 8), ln, bt, 4, 1)
-    for keep, recent in ((0, 0), (4, 5), (4, -1)):
+    for keep, recent in ((0, 0), (4, 5), (4, -1), (2 ** 31, 0), (2 ** 32 + 4, 1)):
         with pytest.raises(E, match="keep"):
             pkg.kv_evict(pool, pool, torch.zeros(2, 2, 8), ln, bt, keep, recent)
