@@ -20,7 +20,10 @@
 // PV (m16n8k16, f16, out^T = V^T P^T: A = V codes, 16 dims; B = P^T, 8 heads).  Heads are the
 // columns of both products, so no MMA row is wasted on a small group, and a lane's
 // score and output columns are the same two heads.  movmatrix turns the score tile into
-// the B operand; a prmt pairs the codes of two tokens, then the same masks apply.  The
+// the B operand; a prmt pairs the codes of two tokens.  Of the two codes in a byte the low one
+// is masked out and the high one taken together with it (c0 + 16 c1, also linear in an
+// f16's bits): sum r c1 = (sum r (c0 + 16 c1) - sum r c0) / 16 loses nothing, the division
+// by 16 shrinking the larger sum's rounding as well, and saves a mask.  The
 // probabilities carry the V scale, r = f16(p s_g):  out = sum_t r c + sum_t p m.  Half a step
 // of r is 2^-11, an eighth of a bf16 output's (1.8e-3 off in all, 1.7e-3 of it the
 // output's).  An f16 output rounds as finely as r does, so for those r is two f16 (the second
@@ -481,8 +484,8 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
     }
 
     // out^T accumulators: o[rr][4 grp + k][x] is dim 64 grp + 8 g + k (+ 4 for x >= 2) of head
-    // 8 rr + 2 c + (x & 1), 16 times larger for odd k; vz: sum of p m over this lane's
-    // tokens.  m: running maximum score, ref: what the scores are exponentiated against.
+    // 8 rr + 2 c + (x & 1), for odd k 16 times that and the even dim before it; vz: sum of p m
+    // over this lane's tokens.  m: running maximum score, ref: what the scores are exponentiated against.
     float o[kN][8][4], vz[kN][2][2], m[kN][2], ref[kN][2], l[kN][2];
     // ceil(log2) of the largest V scale or minimum so far; at least -60, so that the sum of
     // p <= 2^75 stays finite over any context (V values all zero)
@@ -696,18 +699,23 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
           const uint32_t x1 = grp ? e1.y : e1.x, y1 = grp ? o1.y : o1.x;
           const uint32_t lo0 = prmt(x0, y0, 0x5410u), hi0 = prmt(x0, y0, 0x7632u);
           const uint32_t lo1 = prmt(x1, y1, 0x5410u), hi1 = prmt(x1, y1, 0x7632u);
+          // k even: the low nibble of a byte; k odd: the whole byte, low + 16 high
+          uint32_t av[4][4] = {{lo0, hi0, lo1, hi1}};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t mask = k & 1 ? 0x00f000f0u : 0x000f000fu;
-            const int sh = k & 2 ? 8 : 0;
+          for (int x = 0; x < 4; ++x) {
+            av[3][x] = prmt(av[0][x], 0u, 0x4341u);
+            av[2][x] = av[3][x] & 0x000f000fu;
+            av[1][x] = av[0][x] & 0x00ff00ffu;
+            av[0][x] &= 0x000f000fu;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int rr = 0; rr < kN; ++rr)
 #pragma unroll
               for (int part = 0; part < kParts; ++part)
-                mma_f16(o[rr][4 * grp + k], (lo0 >> sh) & mask, (hi0 >> sh) & mask,
-                        (lo1 >> sh) & mask, (hi1 >> sh) & mask, pb[part][rr][grp][0],
-                        pb[part][rr][grp][1]);
-          }
+                mma_f16(o[rr][4 * grp + k], av[k][0], av[k][1], av[k][2], av[k][3],
+                        pb[part][rr][grp][0], pb[part][rr][grp][1]);
         }
       }
       __syncwarp();
@@ -749,15 +757,17 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
         }
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
-          // 2^24 undoes the codes' unit, 2^20 that of the codes 16 times larger
+          // 2^24 undoes the codes' unit; an odd dim is its byte's sum less the even one's, / 16
           const float z = vz[rr][grp][x];
           float v[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float unit = k & 1 ? 1048576.f : 16777216.f;
-            v[k] = fmaf(unit, o[rr][4 * grp + k][x], z) * inv;
-            v[k + 4] = fmaf(unit, o[rr][4 * grp + k][2 + x], z) * inv;
-          }
+          for (int k = 0; k < 4; k += 2)
+#pragma unroll
+            for (int up = 0; up < 2; ++up) {
+              const float low = o[rr][4 * grp + k][2 * up + x], byte = o[rr][4 * grp + k + 1][2 * up + x];
+              v[k + 4 * up] = fmaf(16777216.f, low, z) * inv;
+              v[k + 4 * up + 1] = fmaf(1048576.f, byte - low, z) * inv;
+            }
           const int d = 64 * grp + 8 * g;
           if (whole) {
             uint32_t *ob = reinterpret_cast<uint32_t *>(

@@ -12,7 +12,8 @@ arithmetic, u = 2^-24, half a step of fp32):
     scale sum_d |q_d| (15 s + |m|) with the tensor core's truncation counted double;
     the exponential adds 2^-21;  out moves by at most (2 e + 2^-20) sum_t w_t |v_t|;
   * accumulating sum r c over n tokens: one rounding (2 u) per MMA and per
-    tile of the running sum, which is at most 15 sum w s:
+    tile of the running sum, which is at most 15 sum w s (odd dims: the difference of sums of at
+    most 255 and 15, divided by 16, so 17):
     (n / 16 + 40) 2 u 32 sum_t w_t s_t, and (n / 2 + 40) 2 u for sum p |m|;
   * the output's own rounding: 2^-8 (bf16) or 2^-11 (f16) of the value, and f16's
     smallest step 2^-25.
