@@ -13,14 +13,17 @@
 // Append: eight lanes per row of 128 dims, 16 dims a lane: two 16-byte loads, a two-step
 // shuffle min / max over the 4 lanes of a group, one exchange between the groups' lanes and an
 // 8-byte store (the eight lanes' stores are the row's 64 contiguous bytes).  A CTA takes 16
-// tokens of one head, K and V, so its rows are neighbours in the page.  Issue-bound (31 us
-// for 6211 tokens of 8 heads with a division a value and 8 dims a lane), so the quotient
-// is a multiplication by an approximate 1 / scale, 2^-22 of itself off; a value that this
-// leaves within 2^-16 of a border between two codes is divided, and the codes are
-// always those of the true division.
+// tokens of one head, K and V, so its rows are neighbours in the page.  Issue-bound: 14 us
+// for 6211 tokens of 8 heads (33 MB, 5 us of HBM) at 104 warp instructions a row; 31 us with
+// a division a value and 8 dims a lane.  So the quotient is a multiplication by an
+// approximate 1 / scale, 2^-22 of itself off; a value that this leaves within 2^-16 of a
+// border between two codes is divided, and the codes are always those of the true
+// division.
 //
 // Read-back and widening: eight lanes per row, each with the 8 bytes that hold 8 dims
-// of either group, so that the 16-byte stores of a row are contiguous.
+// of either group, so that the 16-byte stores of a row are contiguous.  Bound by the
+// latency of the small loads (widening 4 rows of 16,000 tokens in all, 8 heads: 20 us for
+// 86 MB), so all of a thread's rows are loaded before the first is stored (30 us without).
 #include "common.cuh"
 #include "int4_page.cuh"
 
@@ -131,8 +134,9 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = 0.f;
   if (live) {
-    const T *src = (is_v ? value + t * value_stride + h * value_head : key + t * key_stride + h * key_head) +
-                   sub * 16;
+    const T *src = is_v ? value + t * value_stride + h * value_head
+                        : key + t * key_stride + h * key_head;
+    src += sub * 16;
     load8<T, kVec>(src, x);
     load8<T, kVec>(src + 8, x + 8);
   }

@@ -4,43 +4,49 @@
 //   S[h, t] = scale * sum_g ( sK_tg (q . c)_g + mK_tg (sum_d q)_g )
 //   out[h]  = sum_t p_t V[t] / sum_t p_t,  p_t = 2^(S log2(e) - running max)
 //
-// The codes go to the tensor cores as they are and scale and minimum are applied to
-// the 8 x 8 score tile and to the probabilities instead of to the 128 dims: that is
-// 4 FMAs a score instead of 64 a token, and no 4-bit value is ever rounded.
+// Bound by HBM in principle (144 bytes a token and head, 4 G 128 FMA) and by issue and ALU
+// slots in fact: unpacking a code costs more than loading it.  So the codes go to the
+// tensor cores as they are, scale and minimum are applied to the score tile and to the
+// probabilities instead of to the 128 dims, and no code is ever rounded.
+// Measured: 128 sequences of 1,024-8,192 tokens, 8 KV heads of 4, bf16: 114 us = 5.98 TB/s
+// at 1,965 MHz (93 % of the copy rate), 136 us in a loop of seconds under the 1,000 W cap;
+// 15 warp instructions a token and head (K and V), half of them ALU.
 //
-// The minimum's term of the scores is one bf16 MMA for 16 tokens: the parameter words are its
-// A operand as they lie in the page.
+// QK^T (m16n8k16, f16, S^T = K q^T: A = K codes, 16 tokens; B = q, 8 heads).  A code in bits
+// 0-3 of an f16 is the subnormal c 2^-24, in bits 4-7 it is 16 c 2^-24: two masks and one
+// shift turn a word of 8 codes into four f16x2 operands, exactly.  q rows are brought to
+// 2^14 <= max |q| < 2^15 by a power of two (the dims that meet the 16 c codes to a
+// sixteenth of that), which the fp32 result undoes with the 2^24.  The minimum's term is
+// one bf16 MMA for 16 tokens: the parameter words are its A operand as they lie in the
+// page, q's group sums in three bf16 pieces its B.
 //
-// QK^T (m16n8k16, f16, S^T = K q^T: A = K codes, 16 tokens; B = q, 8 heads).  A 4-bit code
-// in bits 0-3 of an f16 is the subnormal c 2^-24, in bits 4-7 it is 16 c 2^-24: two masks
-// and one shift turn a word of 8 codes into four f16x2 operands, exactly.  q rows are
-// brought to 2^14 <= max |q| < 2^15 by a power of two (the dims that meet the 16 c
-// codes to a sixteenth of that), which the fp32 result undoes with the 2^24.
-//
-// PV (m16n8k16, f16, out^T = V^T P^T: A = V codes, 16 dims; B = P^T, 8 heads).  Heads are the
-// columns of both products, so no MMA row is wasted on a small group, and a lane's
-// score and output columns are the same two heads.  movmatrix turns the score tile into
-// the B operand; a prmt pairs the codes of two tokens.  Of the two codes in a byte the low one
+// PV (m16n8k16, f16, out^T = V^T P^T: A = V codes, 16 dims; B = P^T, 8 heads).  Heads are
+// the columns of both products, so no MMA row is wasted on a small group, and a lane's
+// score and output columns are the same two heads.  movmatrix turns the score tile into the
+// B operand; a prmt pairs the codes of two tokens.  Of the two codes in a byte the low one
 // is masked out and the high one taken together with it (c0 + 16 c1, also linear in an
 // f16's bits): sum r c1 = (sum r (c0 + 16 c1) - sum r c0) / 16 loses nothing, the division
-// by 16 shrinking the larger sum's rounding as well, and saves a mask.  The
-// probabilities carry the V scale, r = f16(p s_g):  out = sum_t r c + sum_t p m.  Half a step
-// of r is 2^-11, an eighth of a bf16 output's (1.8e-3 off in all, 1.7e-3 of it the
-// output's).  An f16 output rounds as finely as r does, so for those r is two f16 (the second
-// takes what the first leaves) and the product runs twice: 2.1e-4 off, the output's own,
-// instead of 5e-4 with one.  f16 has 5 exponent bits and the scales' range is fp32's: the
-// reference that the scores are exponentiated against is not the running maximum but lies
-// 15 - ceil(log2 max(s, |m|)) below it, the maximum over the tokens seen so far.  r is then
-// at most 2^15 and keeps its 11 bits down to 2^-29 of the largest value (or of 2^-60, if
-// that is more); the sum of p is taken against the same reference, so the quotient does not
-// see it.
+// by 16 shrinking the larger sum's rounding as well, and saves a mask (116 -> 114 us).
+//
+// The probabilities carry the V scale, r = f16(p s_g):  out = sum_t r c + sum_t p m.  Half
+// a step of r is 2^-11, an eighth of a bf16 output's (1.8e-3 off in all, 1.7e-3 of it the
+// output's).  An f16 output rounds as finely as r does, so for those r is two f16 (the
+// second takes what the first leaves) and the product runs twice: 2.1e-4 off, the output's
+// own, instead of 5e-4 with one, at 136 us instead of 117 (both in the same run).  f16
+// has 5 exponent bits and the scales' range is fp32's: the reference that the scores are
+// exponentiated against is not the running maximum but lies 15 - ceil(log2 max(s, |m|))
+// below it, the maximum over the tokens seen so far.  r is then at most 2^15 and keeps
+// its 11 bits down to 2^-29 of the largest value (or of 2^-60, if that is more); the sum
+// of p is taken against the same reference, so the quotient does not see it.
 //
 // Work split: the 64-token tiles of all (sequence, kv head) segments, in that order, cut
 // into equal contiguous ranges, one per warp slot; slot s is warp s / grid of CTA s % grid,
 // so that a few tiles still use every SM.  A segment inside one range is finished in place,
 // the others leave (reference, sum, acc) partials that the merge kernel combines.  Each
 // warp owns a ring of 9,216-byte stages; lane 0 issues two bulk copies a tile (K and V
-// tile are contiguous), with the next page's block id loaded a page ahead.
+// tile are contiguous), with the next page's block id loaded a page ahead.  12 warps with two
+// stages: 8 with three took 131 us instead of 122 then, 16 with K and V tiles apart (128
+// registers, spills) 139 instead of 116.
 #include "common.cuh"
 #include "decode_worklist.cuh"
 #include "int4_page.cuh"
@@ -109,9 +115,15 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 }
 
 // Shared-memory loads as plain C++, which the compiler may schedule between the waits.
-__device__ __forceinline__ uint4 lds128(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
-__device__ __forceinline__ uint32_t lds32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
-__device__ __forceinline__ uint2 lds64(const uint8_t *p) { return *reinterpret_cast<const uint2 *>(p); }
+__device__ __forceinline__ uint4 lds128(const uint8_t *p) {
+  return *reinterpret_cast<const uint4 *>(p);
+}
+__device__ __forceinline__ uint2 lds64(const uint8_t *p) {
+  return *reinterpret_cast<const uint2 *>(p);
+}
+__device__ __forceinline__ uint32_t lds32(const uint8_t *p) {
+  return *reinterpret_cast<const uint32_t *>(p);
+}
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t d;
@@ -485,7 +497,8 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
 
     // out^T accumulators: o[rr][4 grp + k][x] is dim 64 grp + 8 g + k (+ 4 for x >= 2) of head
     // 8 rr + 2 c + (x & 1), for odd k 16 times that and the even dim before it; vz: sum of p m
-    // over this lane's tokens.  m: running maximum score, ref: what the scores are exponentiated against.
+    // over this lane's tokens.  m: running maximum score, ref: what the scores are
+    // exponentiated against.
     float o[kN][8][4], vz[kN][2][2], m[kN][2], ref[kN][2], l[kN][2];
     // ceil(log2) of the largest V scale or minimum so far; at least -60, so that the sum of
     // p <= 2^75 stays finite over any context (V values all zero)
@@ -534,8 +547,8 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
       int room = 0;
       if constexpr (kScored) {
         room = min(valid, p.logits_stride - j * kTile);
-        lg = p.logits + ((static_cast<int64_t>(r.b) * p.hkv + r.h) * p.logits_stride + j * kTile) * p.logits_heads +
-             2 * c;
+        const int64_t row = (static_cast<int64_t>(r.b) * p.hkv + r.h) * p.logits_stride + j * kTile;
+        lg = p.logits + row * p.logits_heads + 2 * c;
       }
 
       // ---- scores of 64 tokens x 8 kN heads, in the accumulators' unit ----
@@ -587,7 +600,8 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
             for (int rr = 0; rr < kN; ++rr)
               if (tok < room && 8 * rr + 2 * c < G)
                 *reinterpret_cast<float2 *>(lg + tok * p.logits_heads + 8 * rr) =
-                    make_float2(sc[rr][i][2 * row] * unscale[rr][0], sc[rr][i][2 * row + 1] * unscale[rr][1]);
+                    make_float2(sc[rr][i][2 * row] * unscale[rr][0],
+                                sc[rr][i][2 * row + 1] * unscale[rr][1]);
           }
         }
       }
