@@ -8,8 +8,8 @@
 // slots in fact: unpacking a code costs more than loading it.  So the codes go to the
 // tensor cores as they are, scale and minimum are applied to the score tile and to the
 // probabilities instead of to the 128 dims, and no code is ever rounded.
-// Measured: 128 sequences of 1,024-8,192 tokens, 8 KV heads of 4, bf16: 114 us = 5.98 TB/s
-// at 1,965 MHz (93 % of the copy rate), 136 us in a loop of seconds under the 1,000 W cap;
+// Measured: 128 sequences of 1,024-8,192 tokens, 8 KV heads of 4, bf16: 117 us = 5.83 TB/s
+// at 1,965 MHz (90 % of the copy rate), 136-140 us in a loop of seconds under the 1,000 W cap;
 // 15 warp instructions a token and head (K and V), half of them ALU.
 //
 // QK^T (m16n8k16, f16, S^T = K q^T: A = K codes, 16 tokens; B = q, 8 heads).  A code in bits
@@ -32,7 +32,7 @@
 // a step of r is 2^-11, an eighth of a bf16 output's (1.8e-3 off in all, 1.7e-3 of it the
 // output's).  An f16 output rounds as finely as r does, so for those r is two f16 (the
 // second takes what the first leaves) and the product runs twice: 2.1e-4 off, the output's
-// own, instead of 5e-4 with one, at 136 us instead of 117 (both in the same run).  f16
+// own, instead of 5e-4 with one, at 136 us instead of 117.  f16
 // has 5 exponent bits and the scales' range is fp32's: the reference that the scores are
 // exponentiated against is not the running maximum but lies 15 - ceil(log2 max(s, |m|))
 // below it, the maximum over the tokens seen so far.  r is then at most 2^15 and keeps
@@ -72,6 +72,7 @@ constexpr int kTile = kv4::kTileTokens;
 constexpr int kStages = 2;
 constexpr int kStage = 2 * kTileBytes;                    // K tile, V tile
 
+constexpr int kFlush = 8;                                 // tiles between two moves out of o
 constexpr int kSkip = 4;                                  // sequences per entry of the tile prefix
 
 // Warps of a CTA by the query-head columns (kN x 8): twice the accumulators at kN = 2 need
@@ -499,7 +500,9 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
     // 8 rr + 2 c + (x & 1), for odd k 16 times that and the even dim before it; vz: sum of p m
     // over this lane's tokens.  m: running maximum score, ref: what the scores are
     // exponentiated against.
-    float o[kN][8][4], vz[kN][2][2], m[kN][2], ref[kN][2], l[kN][2];
+    // moved_o: what was moved out of o, per group and head: the sums are o + moved_o (byte
+    // sums o + 17 moved_o).
+    float o[kN][8][4], vz[kN][2][2], moved_o[kN][2][2], m[kN][2], ref[kN][2], l[kN][2];
     // ceil(log2) of the largest V scale or minimum so far; at least -60, so that the sum of
     // p <= 2^75 stays finite over any context (V values all zero)
     int sexp = -60;
@@ -509,7 +512,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
       for (int n = 0; n < 8; ++n) o[rr][n][0] = o[rr][n][1] = o[rr][n][2] = o[rr][n][3] = 0.f;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        vz[rr][n][0] = vz[rr][n][1] = 0.f;
+        vz[rr][n][0] = vz[rr][n][1] = moved_o[rr][n][0] = moved_o[rr][n][1] = 0.f;
         m[rr][n] = ref[rr][n] = -INFINITY;
         l[rr][n] = 0.f;
       }
@@ -667,6 +670,8 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
           for (int n = 0; n < 2; ++n) {
             vz[rr][n][0] *= alpha[rr][0];
             vz[rr][n][1] *= alpha[rr][1];
+            moved_o[rr][n][0] *= alpha[rr][0];
+            moved_o[rr][n][1] *= alpha[rr][1];
             l[rr][n] *= alpha[rr][n];
           }
         }
@@ -732,6 +737,26 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
                         pb[part][rr][grp][0], pb[part][rr][grp][1]);
         }
       }
+      // The codes are not negative, so o grows with the tokens while out need not, and the
+      // MMA's additions truncate: the mean of 19,000 values in one run was 6.4e-3 off.  Every
+      // kFlush tiles a lane moves the sum of one of its dims out of all of them, which leaves
+      // their differences in o and 2.4e-3 (the output's rounding), for 114 -> 117 us.
+      if ((tt - t) % kFlush == kFlush - 1) {
+#pragma unroll
+        for (int rr = 0; rr < kN; ++rr)
+#pragma unroll
+          for (int grp = 0; grp < 2; ++grp)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float y = o[rr][4 * grp][x];
+              moved_o[rr][grp][x] += y;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int up = 0; up < 2; ++up)
+                  o[rr][4 * grp + k][2 * up + x] = fmaf(k & 1 ? -17.f : -1.f, y, o[rr][4 * grp + k][2 * up + x]);
+            }
+      }
       __syncwarp();
       if (lane == 0 && tt + kStages < e) {
         empty &= ~(1u << stage);
@@ -772,7 +797,7 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
           // 2^24 undoes the codes' unit; an odd dim is its byte's sum less the even one's, / 16
-          const float z = vz[rr][grp][x];
+          const float z = fmaf(16777216.f, moved_o[rr][grp][x], vz[rr][grp][x]);
           float v[8];
 #pragma unroll
           for (int k = 0; k < 4; k += 2)

@@ -11,10 +11,11 @@ arithmetic, u = 2^-24, half a step of fp32):
     products and sums in fp32, each within u of their absolute sum, so e <= 400 u
     scale sum_d |q_d| (15 s + |m|) with the tensor core's truncation counted double;
     the exponential adds 2^-21;  out moves by at most (2 e + 2^-20) sum_t w_t |v_t|;
-  * accumulating sum r c over n tokens: one rounding (2 u) per MMA and per
-    tile of the running sum, which is at most 15 sum w s (odd dims: the difference of sums of at
-    most 255 and 15, divided by 16, so 17):
-    (n / 16 + 40) 2 u 32 sum_t w_t s_t, and (n / 2 + 40) 2 u for sum p |m|;
+  * accumulating sum r c over n tokens: one rounding (2 u, the MMA truncates) per 16 tokens
+    and per tile of a running sum that is moved out every 512 tokens, and so at most 15 times
+    these tokens' sum w s (odd dims: the difference of sums of at most 255 and 15, divided
+    by 16, so 17); the moves add u of the whole each: ((512 / 16 + 40) 2 u 32 + (n / 512 +
+    2) u 17) sum_t w_t s_t; and (n / 8 + 40) 2 u for a lane's sum p |m|;
   * the output's own rounding: 2^-8 (bf16) or 2^-11 (f16) of the value, and f16's
     smallest step 2^-25.
 """
@@ -77,7 +78,7 @@ def decode_bound(q, k, v, ks, vs, kmin_abs, w, out, scale, dtype):
     else:
         b = 2.0 ** -11 * wc
     b = b + (2 * e + 2.0 ** -20).unsqueeze(-1) * wv
-    b = b + (n / 16 + 40) * 2 * U * 32 * ws + (n / 2 + 40) * 2 * U * wz
+    b = b + ((512 / 16 + 40) * 2 * U * 32 + (n / 512 + 2) * U * 17) * ws + (n / 8 + 40) * 2 * U * wz
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
     return b + half * (out.abs() + b) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
 
@@ -350,6 +351,23 @@ def test_decode_values_all_zero(pkg):
     vp[nb - 1] = one[0]
     out = pkg.flash_attn_with_kvcache_int4(q.cuda(), kp, vp, ln, tables.cuda())
     check_decode(out, q, kp, vp, [n], tables, 128 ** -0.5)
+
+
+def test_decode_long_uniform_attention(pkg):
+    """The mean of 19,000 random V rows, each head's in one warp's long run: the result is a
+    hundredth of a value, the sums of codes behind it are not.  Root mean square error of it: the
+    output's rounding (2^-8 / sqrt 3), the rounding of p s against codes of 2.5 times a value
+    (2^-11 2.5 / sqrt 3) and a tenth of that for the sums: 2.4e-3 in all, at most 3e-3."""
+    bs, H, G, n, B = 256, 8, 4, 19000, 128
+    nb = (n + bs - 1) // bs
+    kp, vp = make_pool(pkg, 68, nb, bs, H), make_pool(pkg, 69, nb, bs, H)
+    tables = torch.arange(nb, dtype=torch.int32).repeat(B, 1)          # all rows read the same pages
+    q = torch.zeros(B, 1, H * G, 128, dtype=torch.bfloat16)
+    out = pkg.flash_attn_with_kvcache_int4(q.cuda(), kp, vp, torch.full((B,), n, dtype=torch.int32).cuda(),
+                                           tables.cuda()).cpu().double()
+    ref = R.decode_pool(vp.cpu())[0].reshape(-1, H, 128)[:n].mean(0).repeat_interleave(G, 0)
+    err = (out[:, 0] - ref).square().mean().sqrt() / ref.square().mean().sqrt()
+    assert err <= 3e-3, err
 
 
 def test_decode_nan_stays_in_its_group(pkg):
