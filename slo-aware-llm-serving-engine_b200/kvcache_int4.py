@@ -19,12 +19,13 @@ import torch
 
 from . import _lib
 from ._lib import SlokvError, buffers, check, lib, on_device, require_cuda
-from .kvcache import _i32_contig, _varlen_attention
+from .kvcache import _i32_contig
 
 HEAD_DIM = 128
 TILE_TOKENS = 64
 ROW_BYTES = 72          # 64 bytes of codes, 2 x (scale, minimum) in bf16
 _WIDE_PAGE = 128        # tokens of a page that rows are widened to for prefill
+_WIDE_BYTES = 1 << 30   # scratch of widened rows; more rows than fit run in groups
 
 # A prefill call of at most SHORT_CHUNK query tokens a row, or SHORT_CALL in all, runs as
 # decode rows (8 KV heads of 4, us, prefill / decode rows, L cached tokens: 1 row of 64
@@ -214,8 +215,9 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
     Arguments as flash_attn_varlen_func's paged form, any block_size that the pool
     allows.  Short calls (SHORT_CHUNK, SHORT_CALL) run as decode rows, one a query
     token.  For longer ones the rows' cached tokens are widened once to q's type (one
-    rounding) in a scratch of rows x ceil(max_seqlen_k / 128) pages, which the tcgen05
-    prefill then reads: a few per cent of its time when a chunk is a thousand tokens.
+    rounding) in a scratch of at most 1 GiB (or one row of max_seqlen_k tokens), as many
+    rows at a time as fit, which the tcgen05 prefill then reads: a few per cent of its
+    time when a chunk is a thousand tokens.
     """
     if block_table is None:
         raise SlokvError("4-bit varlen attention reads the pool: block_table is required")
@@ -263,14 +265,28 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
                                table_rows=table_rows)
         return out
     pages = max(1, (max_seqlen_k + _WIDE_PAGE - 1) // _WIDE_PAGE)
+    scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
+    dtype, err = _Q_DTYPES[q.dtype], buffers.error_word(dev).data_ptr()
+    row_bytes = 2 * pages * _WIDE_PAGE * Hkv * HEAD_DIM * q.element_size()
+    group = min(rows, max(1, _WIDE_BYTES // row_bytes))
     with on_device(dev) as stream:
-        wide = torch.empty(2, rows * pages, _WIDE_PAGE, Hkv, HEAD_DIM, dtype=q.dtype, device=dev)
-        table = torch.empty(rows, pages, dtype=torch.int32, device=dev)
-        check(lib().slokv_int4_rows_widen(
-            k_cache.data_ptr(), v_cache.data_ptr(), k_block, v_block, NB, bs, Hkv, HEAD_DIM,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-            cu_seqlens_k.data_ptr(), rows, pages, wide[0].data_ptr(), wide[1].data_ptr(),
-            table.data_ptr(), _Q_DTYPES[q.dtype], buffers.error_word(dev).data_ptr(), stream),
-            "int4_rows_widen")
-        return _varlen_attention(q, wide[0], wide[1], cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
-                                 softmax_scale, causal, table, out, None)
+        wide = torch.empty(2, group * pages, _WIDE_PAGE, Hkv, HEAD_DIM, dtype=q.dtype, device=dev)
+        order = lib().slokv_paged_prefill_workspace_bytes(group, max_seqlen_q)
+        scratch = torch.empty(4 * group * pages + order + 256, dtype=torch.uint8, device=dev)
+        k_wide, v_wide, block = wide[0].data_ptr(), wide[1].data_ptr(), wide.stride(1)
+        work = (scratch.data_ptr() + 255) // 256 * 256
+        table = work + order
+        for r in range(0, rows, group):      # several groups of rows share the scratch in turn
+            n = min(group, rows - r)
+            cu_q, cu_k = cu_seqlens_q.data_ptr() + 4 * r, cu_seqlens_k.data_ptr() + 4 * r
+            check(lib().slokv_int4_rows_widen(
+                k_cache.data_ptr(), v_cache.data_ptr(), k_block, v_block, NB, bs, Hkv, HEAD_DIM,
+                block_table.data_ptr() + 4 * r * block_table.stride(0), block_table.stride(0),
+                block_table.shape[1], cu_k, n, pages, k_wide, v_wide, table, dtype, err, stream),
+                "int4_rows_widen")
+            check(lib().slokv_paged_prefill(
+                out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0),
+                q.stride(1), Tq, k_wide, v_wide, 0, 0, 0, block, block, cu_q, cu_k, n,
+                max_seqlen_q, table, pages, pages, group * pages, _WIDE_PAGE, Hq, Hkv, HEAD_DIM,
+                scale, dtype, None, work, order, err, stream), "paged_prefill")
+    return out

@@ -264,6 +264,47 @@ def test_evict_bad_metadata_is_flagged(pkg):
     assert torch.equal(kp, k0) and torch.equal(vp, v0)
 
 
+def test_evict_captured_and_on_two_streams(pkg):
+    """Two captured evictions replayed side by side, three times on restored inputs, equal the
+    eager ones."""
+    bs, H, keep, recent = 64, 2, 100, 10
+    cases = []
+    for i, lens in enumerate(([300, 90], [700, 101])):
+        nb = sum((n + bs - 1) // bs for n in lens)
+        kp, vp = make_pool(pkg, 81 + i, nb, bs, H), dense_pool(83 + i, nb, bs, H, torch.bfloat16)
+        kp, vp = (kp, kp.clone()) if i else (vp, vp.clone())
+        cases.append([kp, vp, scores_for(85 + i, 2, H, 700, lens, "ties").cuda(),
+                      torch.tensor(lens, dtype=torch.int32).cuda(), make_tables(87 + i, lens, bs, nb).cuda()])
+    start = [[t.clone() for t in c[:3]] for c in cases]
+
+    def restore():
+        for c, s in zip(cases, start):
+            for t, u in zip(c, s):
+                t.copy_(u)
+        torch.cuda.synchronize()
+
+    want = []
+    for c in cases:
+        new, index = pkg.kv_evict(*c, keep, recent, return_index=True)
+        want.append([t.clone() for t in c[:3]] + [new, index])
+    graphs, got = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(pkg.kv_evict(*c, keep, recent, return_index=True))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        restore()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for c, w, (new, index) in zip(cases, want, got):
+            for t, u in zip(c[:3] + [new, index], w):
+                assert torch.equal(t, u)
+
+
 def test_evict_then_attend(pkg):
     """A scored run as it is used: score, evict, decode on.  What remains attends as fp64
     attention over exactly the kept tokens."""

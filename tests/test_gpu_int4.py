@@ -481,6 +481,35 @@ def test_varlen(pkg, qlens, hist, H, G, bs, dtype):
         at += nq
 
 
+def test_varlen_in_groups_and_on_streams(pkg, monkeypatch):
+    """Rows that do not fit the scratch together run in groups; two such calls on two streams
+    at once share nothing."""
+    from importlib import import_module
+    K = import_module("slo-aware-llm-serving-engine_b200.kvcache_int4")
+    H, G, bs, qlens, klens = 2, 4, 64, [70, 5, 0, 90, 33], [300, 5, 10, 700, 40]
+    cases = []
+    for i in range(2):
+        nb = sum((n + bs - 1) // bs for n in klens) + 1
+        kp, vp = make_pool(pkg, 100 + i, nb, bs, H), make_pool(pkg, 102 + i, nb, bs, H)
+        q = torch.from_numpy(det_normal(104 + i, (sum(qlens), H * G, 128))).float().bfloat16().cuda()
+        cu = lambda x: torch.tensor([0] + list(np.cumsum(x)), dtype=torch.int32).cuda()
+        cases.append(((q, kp, vp, cu(qlens), cu(klens), 90, 700),
+                      dict(block_table=make_tables(106 + i, klens, bs, nb).cuda())))
+    whole = [pkg.flash_attn_varlen_func_int4(*a, **k) for a, k in cases]
+    monkeypatch.setattr(K, "_WIDE_BYTES", 2 * 2 * 768 * H * 128 * 2 + 1)      # two rows
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = []
+    for _ in range(10):
+        for (a, k), s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                outs.append(pkg.flash_attn_varlen_func_int4(*a, **k))
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, whole[i % 2])
+    assert pkg.read_device_errors() == 0
+
+
 @pytest.mark.parametrize("nq", [2, 70])
 def test_varlen_bad_metadata_is_flagged(pkg, nq):
     kp, vp = make_pool(pkg, 95, 4, 64, 1), make_pool(pkg, 96, 4, 64, 1)
