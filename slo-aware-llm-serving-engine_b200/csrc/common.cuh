@@ -82,6 +82,19 @@ __device__ __forceinline__ uint64_t l2_evict_first_policy() {
   return pol;
 }
 
+// L2 policy for data that the stream's next kernel reads (a scored decode's scores).
+__device__ __forceinline__ uint64_t l2_evict_last_policy() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
+}
+
+__device__ __forceinline__ void store_pair(float *p, float x, float y, uint64_t policy) {
+  asm volatile("st.global.L2::cache_hint.v2.f32 [%0], {%1, %2}, %3;" ::"l"(p), "f"(x), "f"(y),
+               "l"(policy)
+               : "memory");
+}
+
 // 4-D tiled TMA load into this CTA's shared memory, completion on `bar`.
 // Coordinates are element indices, innermost first; the destination is this
 // CTA's own shared memory.

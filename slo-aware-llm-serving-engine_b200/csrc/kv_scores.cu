@@ -9,7 +9,8 @@
 // tokens per head, the 4-bit decode the heads of a token side by side (what their
 // accumulators make contiguous); both are read here.  The kernel may start before those
 // that store them have ended, so what they store is loaded through L2 (__ldcg) and not
-// through the read-only path.  Bound by the latency of its loads, largely from L2: 21 us
+// through the read-only path.  They are stored to stay in L2 and loaded to leave it (447
+// -> 443 us for the scored decode below).  Bound by the latency of its loads, largely from L2: 21 us
 // for 256 x 8 heads of 512-4,096 tokens (G 4, 113 MB).
 #include "common.cuh"
 
@@ -39,6 +40,22 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// The scores' last use: their lines may go first.
+__device__ __forceinline__ float4 load_last4(const float *p, uint64_t policy) {
+  float4 v;
+  asm volatile("ld.global.cg.L2::cache_hint.v4.f32 {%0, %1, %2, %3}, [%4], %5;"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "l"(p), "l"(policy));
+  return v;
+}
+__device__ __forceinline__ float2 load_last2(const float *p, uint64_t policy) {
+  float2 v;
+  asm volatile("ld.global.cg.L2::cache_hint.v2.f32 {%0, %1}, [%2], %3;"
+               : "=f"(v.x), "=f"(v.y)
+               : "l"(p), "l"(policy));
+  return v;
+}
+
 // kPairs: logits are [batch, hkv, logits_stride, group padded to even]; else [batch, hq,
 // logits_stride], and kVec: score and logit rows allow 16-byte accesses.
 template <bool kPairs, bool kVec>
@@ -59,6 +76,7 @@ __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const Sc
   const int64_t pair = static_cast<int64_t>(b) * p.hkv + h;
   const float *lse = p.lse + pair * p.group;
   float *score = p.scores + row * p.row_stride + h * p.head_stride;
+  const uint64_t last = l2_evict_first_policy();
   if constexpr (kPairs) {
     // a warp's lanes take neighbouring tokens, whose heads lie side by side
     const int32_t heads = (p.group + 1) / 2 * 2;
@@ -79,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const Sc
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (t0 + i * kThreads < len) {
-          const float2 x = __ldcg(reinterpret_cast<const float2 *>(lg + i * step + g));
+          const float2 x = load_last2(lg + i * step + g, last);
           if (d0 != -INFINITY) w[i] += exp2_fast(x.x - d0);
           if (d1 != -INFINITY) w[i] += exp2_fast(x.y - d1);
         }
@@ -102,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) kv_scores_accumulate_kernel(const Sc
       if (d == -INFINITY) continue;
       float x[kPer];
       if (kVec && n == kPer) {
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(lg));
+        const float4 v = load_last4(lg, last);
         x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
       } else {
 #pragma unroll

@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
   const uint32_t ring = base + warp * R::kStages * R::kStage;
   const uint32_t bars = bars_all + warp * R::kStages * 8;
   const uint64_t policy = l2_evict_first_policy();
+  const uint64_t keep = kScored ? l2_evict_last_policy() : 0;
   const int tiles_per_block = p.block_size / kTile;
 
   IssueCursor cur;                        // lane 0: next tile to issue (a + issued)
@@ -457,9 +458,9 @@ __global__ void __launch_bounds__(Ring<kFp8>::kWarpsPerCta * 32, 1)
           // rows are a multiple of four floats apart, so a pair is one 8-byte store
 #pragma unroll
           for (int nt = 0; nt < 4; ++nt) {
-            float2 *at = reinterpret_cast<float2 *>(lg + nt * 8 + 2 * c);
-            if (g < G) *at = make_float2(sc[nt][0], sc[nt][1]);
-            if (g + 8 < G) at[4 * p.logits_stride] = make_float2(sc[nt][2], sc[nt][3]);
+            float *at = lg + nt * 8 + 2 * c;
+            if (g < G) store_pair(at, sc[nt][0], sc[nt][1], keep);
+            if (g + 8 < G) store_pair(at + 8 * p.logits_stride, sc[nt][2], sc[nt][3], keep);
           }
         } else {
 #pragma unroll
