@@ -10,8 +10,8 @@
 // accumulators make contiguous); both are read here.  The kernel may start before those
 // that store them have ended, so what they store is loaded through L2 (__ldcg) and not
 // through the read-only path.  They are stored to stay in L2 and loaded to leave it (447
-// -> 443 us for the scored decode below).  Bound by the latency of its loads, largely from L2: 21 us
-// for 256 x 8 heads of 512-4,096 tokens (G 4, 113 MB).
+// -> 439 us for the scored decode below).  Bound by the latency of its loads, largely
+// from L2: 21 us for 256 x 8 heads of 512-4,096 tokens (G 4, 113 MB).
 #include "common.cuh"
 
 namespace slokv {

@@ -8,8 +8,8 @@
 // slots in fact: unpacking a code costs more than loading it.  So the codes go to the
 // tensor cores as they are, scale and minimum are applied to the score tile and to the
 // probabilities instead of to the 128 dims, and no code is ever rounded.
-// Measured: 128 sequences of 1,024-8,192 tokens, 8 KV heads of 4, bf16: 117 us = 5.83 TB/s
-// at 1,965 MHz (90 % of the copy rate), 136-140 us in a loop of seconds under the 1,000 W cap;
+// Measured: 128 sequences of 1,024-8,192 tokens, 8 KV heads of 4, bf16: 118 us = 5.77 TB/s
+// at 1,965 MHz (89 % of the copy rate), 136-140 us in a loop of seconds under the 1,000 W cap;
 // 15 warp instructions a token and head (K and V), half of them ALU.
 //
 // QK^T (m16n8k16, f16, S^T = K q^T: A = K codes, 16 tokens; B = q, 8 heads).  A code in bits
@@ -32,7 +32,7 @@
 // a step of r is 2^-11, an eighth of a bf16 output's (1.8e-3 off in all, 1.7e-3 of it the
 // output's).  An f16 output rounds as finely as r does, so for those r is two f16 (the
 // second takes what the first leaves) and the product runs twice: 2.1e-4 off, the output's
-// own, instead of 5e-4 with one, at 136 us instead of 117.  f16
+// own, instead of 5e-4 with one, at 137 us instead of 118.  f16
 // has 5 exponent bits and the scales' range is fp32's: the reference that the scores are
 // exponentiated against is not the running maximum but lies 15 - ceil(log2 max(s, |m|))
 // below it, the maximum over the tokens seen so far.  r is then at most 2^15 and keeps
@@ -266,7 +266,7 @@ struct Cursor {
   int32_t in_page;       // tiles left in the page, this one included
   int32_t b, h, page;    // sequence, kv head, page of the segment
   int32_t left;          // tiles left in the segment, this one included
-  int32_t ahead;         // block id of the page that follows in the order
+  int32_t ahead;         // block id of the page that follows in the range
 };
 
 __device__ __forceinline__ int32_t table_entry(const Params &p, int32_t b, int32_t page) {
@@ -274,10 +274,20 @@ __device__ __forceinline__ int32_t table_entry(const Params &p, int32_t b, int32
   return __ldg(p.block_tables + static_cast<int64_t>(b) * p.bt_stride + page);
 }
 
-// Enter page c.page of segment (c.b, c.h), whose block id is `blk`, at tile `first`, and
-// load the id of the page after it: the segment's next, else the first page of the next
-// segment (0 past the end: it is never used).
-__device__ __forceinline__ void cursor_page(Cursor &c, const Params &p, int32_t blk, int32_t first,
+// The sequence after b that has tokens, whose first tile is tile t of the work list: the
+// neighbour, or behind a gap, however long, the one that the prefix gives.  (140 sequences
+// of 512 tokens padded to 256: 33 us when each warp walks the gap, 29.6 us so; three
+// sequences of 8,192: 323 and 29 us.)
+__device__ __forceinline__ int32_t next_seq(const Params &p, const int32_t *prefix, int32_t b,
+                                            int32_t t) {
+  return seq_len(p, b + 1) ? b + 1 : locate(p, prefix, t).b;
+}
+
+// Enter page c.page of segment (c.b, c.h), whose block id is `blk`, at its tile `first`,
+// tile t of the work list, and load the id of the page after it if the range, which ends
+// at `end`, reaches it: the segment's next, else the first page of the next segment.
+__device__ __forceinline__ void cursor_page(Cursor &c, const Params &p, const int32_t *prefix,
+                                            int32_t blk, int32_t first, int32_t t, int32_t end,
                                             int tiles_per_block) {
   c.k = c.v = nullptr;
   if (blk >= 0 && blk < p.num_blocks) {
@@ -289,29 +299,29 @@ __device__ __forceinline__ void cursor_page(Cursor &c, const Params &p, int32_t 
     record_error(p.err, SLOKV_DEVERR_BLOCK_RANGE);
   }
   c.in_page = min(tiles_per_block - first, c.left);
+  if (t + c.in_page >= end) return;
   int32_t b = c.b, page = c.page + 1;
   if (c.in_page == c.left) {
     page = 0;
-    if (c.h + 1 == p.hkv) {
-      do {
-        ++b;
-      } while (b < p.batch && seq_tiles(p, b) == 0);
-    }
+    if (c.h + 1 == p.hkv) b = next_seq(p, prefix, b, t + c.in_page);
   }
-  c.ahead = b < p.batch ? table_entry(p, b, page) : 0;
+  c.ahead = table_entry(p, b, page);
 }
 
-__device__ __forceinline__ void cursor_init(Cursor &c, const Params &p, const TileRef &r,
+__device__ __forceinline__ void cursor_init(Cursor &c, const Params &p, const int32_t *prefix,
+                                            const TileRef &r, int32_t t, int32_t end,
                                             int tiles_per_block) {
   c.b = r.b;
   c.h = r.h;
   c.page = r.j / tiles_per_block;
   c.left = r.nt - r.j;
-  cursor_page(c, p, table_entry(p, c.b, c.page), r.j - c.page * tiles_per_block, tiles_per_block);
+  cursor_page(c, p, prefix, table_entry(p, c.b, c.page), r.j - c.page * tiles_per_block, t, end,
+              tiles_per_block);
 }
 
-// Step to the following tile; call only when one exists.
-__device__ __forceinline__ void cursor_next(Cursor &c, const Params &p, int tiles_per_block) {
+// Step to the following tile, tile t of the work list; call only if it is in the range.
+__device__ __forceinline__ void cursor_next(Cursor &c, const Params &p, const int32_t *prefix,
+                                            int32_t t, int32_t end, int tiles_per_block) {
   --c.left;
   if (--c.in_page) {
     if (c.k) {
@@ -325,14 +335,11 @@ __device__ __forceinline__ void cursor_next(Cursor &c, const Params &p, int tile
     c.page = 0;
     if (++c.h == p.hkv) {
       c.h = 0;
-      do {
-        c.left = seq_tiles(p, ++c.b);
-      } while (c.left == 0 && c.b + 1 < p.batch);
-    } else {
-      c.left = seq_tiles(p, c.b);
+      c.b = next_seq(p, prefix, c.b, t);
     }
+    c.left = seq_tiles(p, c.b);
   }
-  cursor_page(c, p, c.ahead, 0, tiles_per_block);
+  cursor_page(c, p, prefix, c.ahead, 0, t, end, tiles_per_block);
 }
 
 // Issue the copies of the cursor's tile into `stage`.  A page outside the pool is not
@@ -408,10 +415,10 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
   Cursor cur = {};                  // lane 0: the tile that is issued next
   uint32_t empty = 0;               // lane 0: stages whose page lies outside the pool
   if (lane == 0) {
-    cursor_init(cur, p, r, tiles_per_block);
+    cursor_init(cur, p, prefix, r, a, e, tiles_per_block);
     for (int i = 0; i < kStages && a + i < e; ++i) {
       if (!issue_tile(cur, ring, bars, i, policy)) empty |= 1u << i;
-      if (a + i + 1 < e) cursor_next(cur, p, tiles_per_block);
+      if (a + i + 1 < e) cursor_next(cur, p, prefix, a + i + 1, e, tiles_per_block);
     }
   }
   __syncwarp();
@@ -762,7 +769,9 @@ __global__ void __launch_bounds__(warps_of(kN) * 32, 1) paged_decode_int4_kernel
       if (lane == 0 && tt + kStages < e) {
         empty &= ~(1u << stage);
         if (!issue_tile(cur, ring, bars, stage, policy)) empty |= 1u << stage;
-        if (tt + kStages + 1 < e) cursor_next(cur, p, tiles_per_block);
+        if (tt + kStages + 1 < e) {
+          cursor_next(cur, p, prefix, tt + kStages + 1, e, tiles_per_block);
+        }
       }
       __syncwarp();
     }

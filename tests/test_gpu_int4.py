@@ -244,6 +244,23 @@ def test_decode_many_rows_and_batch_prefix(pkg):
         check_decode(out, q, kp, vp, lens, tables, scale)
 
 
+def test_decode_batch_limit_and_long_gaps(pkg):
+    """8,192 rows, all but three without tokens, one of them long: ranges cross the gaps."""
+    bs, H, G, B = 64, 1, 1, 8192
+    lens = [0] * B
+    lens[5], lens[4000], lens[8191] = 130, 20000, 65
+    nb = sum((n + bs - 1) // bs for n in lens)
+    kp, vp = make_pool(pkg, 25, nb, bs, H), make_pool(pkg, 26, nb, bs, H)
+    short = make_tables(27, [130, 20000, 65], bs, nb)
+    tables = torch.full((B, short.shape[1]), -1, dtype=torch.int32)
+    tables[[5, 4000, 8191]] = short
+    q = torch.from_numpy(det_normal(28, (B, 1, 1, 128))).float().bfloat16()
+    out = pkg.flash_attn_with_kvcache_int4(q.cuda(), kp, vp, torch.tensor(lens, dtype=torch.int32).cuda(),
+                                           tables.cuda())
+    check_decode(out, q, kp, vp, lens, tables, 128 ** -0.5)
+    assert pkg.read_device_errors() == 0
+
+
 def test_decode_stale_and_foreign_bytes(pkg):
     """0xFF bytes (NaN parameters) in every slot that no sequence reaches change nothing."""
     lens, bs, H, G = [65, 130, 1], 128, 2, 4
