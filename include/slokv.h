@@ -448,9 +448,10 @@ int slokv_int4_rows_widen(const void *k_cache, const void *v_cache, int64_t k_bl
 
 /* Paged decode over a 4-bit pool: slokv_paged_decode's arguments and result with
  * the pool as above.  q / out are bf16 or f16 (q_dtype), at most 16 query heads per
- * KV head, batch at most 8192.  table_rows: NULL, or the block table row of each
- * sequence; with it a context length of -1 leaves the sequence's output unwritten
- * (slokv_int4_rows_expand).  logits / lse: NULL, or both as for a scored decode (below),
+ * KV head, batch at most 8192, batch * num_kv_heads * the table's reach in tiles of 64
+ * tokens below 2^31 (else SLOKV_ERR_UNSUPPORTED).  table_rows: NULL, or the block
+ * table row of each sequence; with it a context length of -1 leaves the sequence's
+ * output unwritten (slokv_int4_rows_expand).  logits / lse: NULL, or both as for a scored decode (below),
  * logits being [batch, num_kv_heads, logits_stride, group rounded up to even] fp32, 8-byte
  * aligned.  The workspace holds nothing between calls. */
 size_t slokv_paged_decode_int4_workspace_bytes(int32_t device, int32_t num_q_heads,
@@ -463,8 +464,8 @@ int slokv_paged_decode_int4(void *out, int64_t out_stride_b, int64_t out_stride_
                             int64_t block_table_stride, int32_t max_blocks_per_seq,
                             const int32_t *table_rows, const int32_t *context_lens,
                             int32_t batch, float softmax_scale, int32_t q_dtype, float *logits,
-                            int64_t logits_stride, float *lse, void *workspace, size_t workspace_bytes, uint32_t *dev_error,
-                            void *stream);
+                            int64_t logits_stride, float *lse, void *workspace,
+                            size_t workspace_bytes, uint32_t *dev_error, void *stream);
 
 /* The queries of a short prefill chunk as decode rows: for query token t of row r
  * (cu_seqlens_q[r] <= t < cu_seqlens_q[r + 1]), table_rows[t] = r and context_lens[t] =
@@ -484,7 +485,8 @@ int slokv_int4_rows_expand(const int32_t *cu_seqlens_q, const int32_t *cu_seqlen
  *   lse[b, hq] = log2 sum_t 2^logits[b, hq, t]
  * slokv_paged_decode_logits: slokv_paged_decode (bf16 / f16 pools) plus logits
  * ([batch, num_q_heads, logits_stride] fp32, 16-byte aligned, logits_stride a multiple of
- * 4) and lse ([batch, num_q_heads] fp32).
+ * 4) and lse ([batch, num_q_heads] fp32); batch * num_kv_heads * the table's reach in
+ * tiles of 32 tokens below 2^31.
  */
 int slokv_paged_decode_logits(void *out, int64_t out_stride_b, int64_t out_stride_h, const void *q,
                               int64_t q_stride_b, int64_t q_stride_h, const void *k_cache,
@@ -505,6 +507,7 @@ int slokv_paged_decode_logits(void *out, int64_t out_stride_b, int64_t out_strid
  * SLOKV_DEVERR_SLOT_RANGE; two sequences of one call must not share a row.  Positions
  * past min(width, logits_stride, max_context) are left alone, with
  * SLOKV_DEVERR_CONTEXT_LEN; max_context: the decode's max_blocks_per_seq * block_size.
+ * That minimum is at most 2^30 (else SLOKV_ERR_UNSUPPORTED).
  * logits_pairs: 0 for slokv_paged_decode_logits' layout, 1 for slokv_paged_decode_int4's. */
 int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int64_t head_stride,
                                int32_t width, int32_t num_score_rows, const int32_t *score_rows,

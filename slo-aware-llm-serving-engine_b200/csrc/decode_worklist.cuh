@@ -14,6 +14,13 @@ constexpr int kRowFloats = kD + 4;              // partial row: m, l, pad, pad, 
 constexpr int kAccOff = 4;                      // acc starts 16-byte aligned
 constexpr int kMaxBatch = 8192;
 
+// Whether the work list of every table row filled to its reach counts in 32 bits.
+inline bool tiles_fit(int64_t batch, int64_t hkv, int64_t max_blocks, int64_t block_size, int tile) {
+  const int64_t segments = batch * hkv;
+  return segments <= 0x7fffffff &&
+         (max_blocks * block_size + tile - 1) / tile <= 0x7fffffff / segments;
+}
+
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -378,7 +378,7 @@ extern "C" int slokv_kv_evict(void *k_cache, void *v_cache, int64_t k_block_stri
   if (score_width < cap) cap = score_width;
   const int64_t most = most_moves(keep, cap);
   const int64_t chunks = (most + kMovesPerCta - 1) / kMovesPerCta;
-  if (pairs > 0x7fffffff || chunks > 65535) return SLOKV_ERR_UNSUPPORTED;
+  if (pairs > 0x7fffffff || chunks > 65535 || cap > (1 << 30)) return SLOKV_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < evict_workspace(pairs, keep, score_width))
     return SLOKV_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 3u) return SLOKV_ERR_ALIGNMENT;

@@ -182,6 +182,7 @@ extern "C" int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int
   p.decay = decay;
   p.err = dev_error;
   if (cap == 0) return SLOKV_OK;
+  if (cap > (1 << 30)) return SLOKV_ERR_UNSUPPORTED;  // a position plus a CTA's span fits 32 bits
   const bool vec = !((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(logits)) & 15u) &&
                    !((row_stride | head_stride | logits_stride) & 3);
   const dim3 grid(static_cast<unsigned>((cap + kThreads * kPer - 1) / (kThreads * kPer)),

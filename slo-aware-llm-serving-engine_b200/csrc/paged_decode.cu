@@ -1148,6 +1148,10 @@ extern "C" int slokv_paged_decode_logits(void *out, int64_t out_stride_b, int64_
                                          void *stream) {
   if (batch > 0 && (!logits || !lse || logits_stride <= 0)) return SLOKV_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(logits) & 15u) || (logits_stride & 3)) return SLOKV_ERR_ALIGNMENT;
+  if (batch > 0 && num_kv_heads > 0 && max_blocks_per_seq > 0 && block_size > 0 &&
+      !slokv::decode::tiles_fit(batch, num_kv_heads, max_blocks_per_seq, block_size,
+                                slokv::decode::kTile))
+    return SLOKV_ERR_UNSUPPORTED;
   return slokv::decode::run_decode(
       false, out, out_stride_b, out_stride_h, q, q_stride_b, q_stride_h, k_cache, v_cache,
       k_block_stride, v_block_stride, nullptr, nullptr, num_blocks, block_size, num_q_heads,

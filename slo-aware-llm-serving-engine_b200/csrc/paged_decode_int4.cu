@@ -1013,6 +1013,9 @@ extern "C" int slokv_paged_decode_int4(void *out, int64_t out_stride_b, int64_t 
   if (num_q_heads % num_kv_heads) return SLOKV_ERR_INVALID_ARG;
   const int group = num_q_heads / num_kv_heads;
   if (group > 16 || block_size % kTile) return SLOKV_ERR_UNSUPPORTED;
+  if (max_blocks_per_seq > 0 &&
+      !decode::tiles_fit(batch, num_kv_heads, max_blocks_per_seq, block_size, kTile))
+    return SLOKV_ERR_UNSUPPORTED;
   if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens ||
       max_blocks_per_seq <= 0 || (logits != nullptr) != (lse != nullptr))
     return SLOKV_ERR_INVALID_ARG;

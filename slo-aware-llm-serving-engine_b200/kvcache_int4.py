@@ -251,7 +251,8 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
     if block_table.shape[1] == 0:
         raise SlokvError("block_table has no columns")
     if ((max_seqlen_q <= SHORT_CHUNK or Tq <= SHORT_CALL) and Tq <= _MAX_DECODE_ROWS
-            and Hq // Hkv <= _MAX_GROUP):
+            and Hq // Hkv <= _MAX_GROUP
+            and Tq * Hkv * block_table.shape[1] * (bs // TILE_TOKENS) < 2 ** 31):
         scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
         with on_device(dev) as stream:
             nbytes = decode_int4_workspace_bytes(dev.index, Hq, Hkv)

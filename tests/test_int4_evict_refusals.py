@@ -134,3 +134,25 @@ def test_python_refusals(pkg):
     for keep, recent in ((0, 0), (4, 5), (4, -1), (2 ** 31, 0), (2 ** 32 + 4, 1)):
         with pytest.raises(E, match="keep"):
             pkg.kv_evict(pool, pool, torch.zeros(2, 2, 8), ln, bt, keep, recent)
+
+
+def test_sizes_past_32_bits_are_refused(pkg):
+    """A table's reach whose tiles, or a score row whose positions, pass 32 bits."""
+    lib = pkg._lib.lib()
+
+    def int4(batch, hkv, w):
+        stride = hkv * 64 * 72
+        return lib.slokv_paged_decode_int4(P, 1024, 128, P, 1024, 128, P, P, stride, stride, 3, 64, hkv,
+                                           hkv, 128, P, w, w, None, P, batch, 0.1, 0, None, 0, None,
+                                           None, 0, None, None)
+    assert int4(8192, 64, 4096) == -3 and int4(1, 2, 2 ** 30) == -3 and int4(8192, 2 ** 18, 1) == -3
+
+    def logits(batch, w):
+        return lib.slokv_paged_decode_logits(P, 1024, 128, P, 1024, 128, P, P, 32768, 32768, 3, 64, 8, 2,
+                                             128, P, w, w, P, batch, 0.1, 0, P, 64, P, None, 0, None, None)
+    assert logits(8192, 2 ** 16) == -3 and logits(1, 2 ** 29) == -3
+
+    assert lib.slokv_kv_scores_accumulate(P, 2 ** 31, 2 ** 31, 2 ** 31 - 1, 2, None, P, 2 ** 31, 0, P, P, 2,
+                                          8, 2, 2 ** 40, 1.0, None, None) == -3
+    assert lib.slokv_kv_evict(P, P, 32768, 32768, 3, 64, 2, 128, 0, P, 2 ** 26, 2 ** 26, P, 2, P, 2 ** 31,
+                              2 ** 31, 2 ** 31 - 1, 2, None, 10, 4, P, None, P, 2 ** 40, None, None) == -3
