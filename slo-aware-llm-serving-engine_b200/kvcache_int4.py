@@ -53,26 +53,26 @@ def int4_pool_shape(num_blocks: int, block_size: int, num_kv_heads: int):
 def int4_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor):
     """(num_blocks, block_size, num_kv_heads, K and V block strides in bytes) of a 4-bit
     pool, checked."""
-    if k_cache.shape != v_cache.shape:
+    shape = k_cache.shape
+    if v_cache.shape != shape:
         raise SlokvError("k_cache and v_cache shapes differ")
-    strides = []
-    for c in (k_cache, v_cache):
-        if not is_int4_cache(c):
-            raise SlokvError("k_cache / v_cache must be uint8 4-bit pools [num_blocks, "
-                             f"num_kv_heads, block_size * {ROW_BYTES}]")
-        nb, h, size = c.shape
-        if size == 0 or size % (TILE_TOKENS * ROW_BYTES):
-            raise SlokvError(f"a 4-bit pool's last dim must be block_size * {ROW_BYTES} bytes, "
-                             f"block_size a multiple of {TILE_TOKENS}")
-        block, head, one = c.stride()
-        if one != 1 or (h > 1 and head != size):
-            raise SlokvError("a 4-bit pool's blocks must be contiguous")
-        if nb <= 1:
-            block = h * size
-        elif block < h * size:
-            raise SlokvError("a 4-bit pool's blocks must not overlap")
-        strides.append(block)
-    return nb, size // ROW_BYTES, h, strides[0], strides[1]
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or len(shape) != 3:
+        raise SlokvError("k_cache / v_cache must be uint8 4-bit pools [num_blocks, "
+                         f"num_kv_heads, block_size * {ROW_BYTES}]")
+    nb, h, size = shape
+    if size == 0 or size % (TILE_TOKENS * ROW_BYTES):
+        raise SlokvError(f"a 4-bit pool's last dim must be block_size * {ROW_BYTES} bytes, "
+                         f"block_size a multiple of {TILE_TOKENS}")
+    k_block, k_head, k_one = k_cache.stride()
+    v_block, v_head, v_one = v_cache.stride()
+    if k_one != 1 or v_one != 1 or (h > 1 and (k_head != size or v_head != size)):
+        raise SlokvError("a 4-bit pool's blocks must be contiguous")
+    run = h * size
+    if nb <= 1:
+        k_block = v_block = run
+    elif k_block < run or v_block < run:
+        raise SlokvError("a 4-bit pool's blocks must not overlap")
+    return nb, size // ROW_BYTES, h, k_block, v_block
 
 
 def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -130,24 +130,24 @@ def int4_decode(cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
 def check_decode_args(q, cache_seqlens, block_table, out):
     """Argument checks that the paged decodes of this package's 4-bit and scored
     paths share; returns (batch, query heads, out)."""
-    if q.dim() != 4:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 4 or shape[1] != 1 or shape[3] != HEAD_DIM:
         raise SlokvError(f"paged decode expects q of shape [batch, 1, heads, {HEAD_DIM}]")
-    B, one, Hq, D = q.shape
-    if one != 1 or D != HEAD_DIM:
-        raise SlokvError(f"paged decode expects q of shape [batch, 1, heads, {HEAD_DIM}]")
-    if q.dtype not in _Q_DTYPES or q.stride(3) != 1:
+    B, Hq = shape[0], shape[2]
+    if dtype not in _Q_DTYPES or q.stride(3) != 1:
         raise SlokvError("q must be bf16 or f16 with a contiguous last dimension")
     _i32_contig("cache_seqlens", cache_seqlens)
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+    table = block_table.shape
+    if len(table) != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
         raise SlokvError("block_table must be int32 [batch, pages] with a contiguous last dim")
-    rows, width = block_table.shape
+    rows, width = table
     if rows < B or cache_seqlens.numel() < B:
         raise SlokvError("block_table / cache_seqlens have fewer rows than q")
     if width == 0:
         raise SlokvError("block_table has no columns")
     if out is None:
-        out = torch.empty(B, 1, Hq, HEAD_DIM, dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.stride(3) != 1:
+        out = torch.empty(B, 1, Hq, HEAD_DIM, dtype=dtype, device=q.device)
+    elif out.dtype != dtype or out.shape != shape or out.stride(3) != 1:
         raise SlokvError("out must match q's shape and dtype with a contiguous last dim")
     return B, Hq, out
 
