@@ -111,8 +111,9 @@ class KVPool:
             if hasattr(m, "k_cache") and hasattr(m, "v_cache"):
                 m.k_cache = self.kv_cache[0, layer]
                 m.v_cache = self.kv_cache[1, layer]
-                if self.k_scale is not None:
-                    m.k_scale, m.v_scale = self.k_scale[layer], self.v_scale[layer]
+                # None too: a module that held an FP8 pool before would dispatch on its scales
+                m.k_scale = None if self.k_scale is None else self.k_scale[layer]
+                m.v_scale = None if self.v_scale is None else self.v_scale[layer]
                 layer += 1
         if layer != self.num_layers:
             raise RuntimeError(f"bound {layer} attention layers, pool has {self.num_layers}")
