@@ -238,6 +238,7 @@ class GreedyRunner:
                                       self.W * block_size, dtype=torch.float32, device=dev)
         for i, attn in enumerate(model.attention_modules()):
             attn.scores = None if self.scores is None else self.scores[i]
+            attn.score_rows, attn.score_decay = None, 1.0   # an earlier user's map and decay go too
 
     def _slots(self, b: int, start: int, stop: int) -> list[int]:
         row = self.tables[b].tolist()
