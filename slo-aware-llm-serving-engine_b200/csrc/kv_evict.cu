@@ -82,8 +82,9 @@ __global__ void __launch_bounds__(kThreads) kv_evict_select_kernel(const EvictPa
     p.new_lens[b] = known && fits && n > p.keep ? p.keep : n;
   }
   int32_t *index = p.index ? p.index + static_cast<int64_t>(blockIdx.x) * p.keep : nullptr;
-  if (index)
-    for (int32_t i = tid; i < p.keep; i += kThreads) index[i] = i < n ? i : -1;
+  if (index)   // unsigned: keep may be 2^31 - 1, and a signed i would wrap below it
+    for (uint32_t i = tid; i < static_cast<uint32_t>(p.keep); i += kThreads)
+      index[i] = static_cast<int32_t>(i) < n ? static_cast<int32_t>(i) : -1;
   if (!known || !fits || n <= p.keep) {
     if (tid == 0) p.counts[blockIdx.x] = 0;
     return;

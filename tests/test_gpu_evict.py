@@ -327,3 +327,22 @@ def test_evict_then_attend(pkg):
         # 2^-8 for the bf16 output, 2^-11 for the rounded probabilities of values up to 4
         assert ((out[0, 0, h * G:(h + 1) * G] - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -11 * 4).all()
     assert (scores[0, :, keep:] == 0).all()
+
+
+def test_evict_index_up_to_the_largest_keep(pkg):
+    """keep 2^31 - 1 (keep everything, 8 GiB of index): the index fill ends with the buffer."""
+    bs, keep, lens = 64, 2 ** 31 - 1, [100, 0]
+    kp, vp = make_pool(pkg, 91, 2, bs, 1), make_pool(pkg, 92, 2, bs, 1)
+    k0 = kp.clone()
+    scores = torch.ones(2, 1, 128, device="cuda")
+    tables = torch.tensor([[0, 1], [1, 0]], dtype=torch.int32, device="cuda")
+    for b in range(2):
+        new, index = pkg.kv_evict(kp, vp, scores[b:b + 1], torch.tensor(lens[b:b + 1], dtype=torch.int32).cuda(),
+                                  tables[b:b + 1], keep, 0, return_index=True)
+        torch.cuda.synchronize()
+        assert new.tolist() == lens[b:b + 1]
+        assert torch.equal(index[0, 0, :lens[b]].cpu(), torch.arange(lens[b], dtype=torch.int32))
+        for at in range(lens[b], keep, 2 ** 29):
+            assert (index[0, 0, at:at + 2 ** 29] == -1).all()
+        del index
+    assert torch.equal(kp, k0) and pkg.read_device_errors() == 0
