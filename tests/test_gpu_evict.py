@@ -346,3 +346,38 @@ def test_evict_index_up_to_the_largest_keep(pkg):
             assert (index[0, 0, at:at + 2 ** 29] == -1).all()
         del index
     assert torch.equal(kp, k0) and pkg.read_device_errors() == 0
+
+
+@pytest.mark.parametrize("kind", ["normal", "ties", "odd", "zeros"])
+def test_evict_past_one_group_of_words_a_warp(pkg, kind):
+    """Rows of more than 32,768 tokens, where a warp ranks several groups of 32 words and
+    carries its ties from one to the next; bytes compared exactly."""
+    bs, H, lens, keep, recent = 256, 2, [41007, 70003, 32769], 9001, 130
+    nb = sum((n + bs - 1) // bs for n in lens)
+    width = max(lens)
+    kp, vp = dense_pool(93, nb, bs, H, torch.bfloat16), dense_pool(94, nb, bs, H, torch.bfloat16)
+    tables = make_tables(95, lens, bs, nb)
+    scores = scores_for(96, 3, H, width, lens, kind)
+    want_s, want_i = scores.clone(), torch.empty(3, H, keep, dtype=torch.int64)
+    for b, n in enumerate(lens):
+        for h in range(H):
+            want_i[b, h] = torch.tensor(R.kept_index(scores[b, h].tolist(), n, keep, recent))
+            want_s[b, h, :keep] = scores[b, h, want_i[b, h]]
+            want_s[b, h, keep:n] = 0
+    want = []
+    for pool in (kp, vp):
+        w, flat = pool.clone(), pool.flatten(0, 1)
+        for b in range(3):
+            t = tables[b].long().cuda()
+            slot = lambda x: t[x // bs] * bs + x % bs
+            for h in range(H):
+                w.flatten(0, 1)[slot(torch.arange(keep).cuda()), h] = flat[slot(want_i[b, h].cuda()), h]
+        want.append(w)
+    gs = scores.cuda()
+    new, index = pkg.kv_evict(kp, vp, gs, torch.tensor(lens, dtype=torch.int32).cuda(), tables.cuda(),
+                              keep, recent, return_index=True)
+    assert new.tolist() == [keep] * 3 and pkg.read_device_errors() == 0
+    assert torch.equal(index.cpu().long(), want_i)
+    assert torch.equal(gs.cpu().view(torch.int32), want_s.view(torch.int32))
+    for pool, w in zip((kp, vp), want):
+        assert torch.equal(pool.view(torch.int16), w.view(torch.int16))
