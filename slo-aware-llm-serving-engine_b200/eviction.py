@@ -91,9 +91,9 @@ def flash_attn_with_kvcache_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cac
       scores[row, h, t] = decay * scores[row, h, t] + sum over h's query heads of softmax[t]
     for every cached position t of each sequence.  decay 1 accumulates, decay 0
     overwrites with this step's weights.  max_seqlen_k (default: scores' width) bounds
-    the context lengths: it sizes the [B, Hq, max_seqlen_k] fp32 scratch, and positions
-    past it or past scores' width are not scored (device error CONTEXT_LEN).  Two
-    sequences of one call must not share a score row; shared blocks are fine.
+    the context lengths: positions past it or past scores' width are not scored (device
+    error CONTEXT_LEN).  The scratch is fp32 [B, Hq, min(max_seqlen_k, the block table's
+    reach)].  Two sequences of one call must not share a score row; shared blocks are fine.
     """
     four = is_int4_cache(k_cache)
     if four:
@@ -115,7 +115,8 @@ def flash_attn_with_kvcache_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     if width <= 0:
         raise SlokvError("scores have no columns (or max_seqlen_k is not positive)")
     scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
-    stride = (width + 3) // 4 * 4
+    reach = block_table.shape[1] * bs
+    stride = (min(width, reach) + 3) // 4 * 4
     with on_device(dev) as stream:
         nbytes = (decode_int4_workspace_bytes if four else _decode_workspace_bytes)(dev.index, Hq,
                                                                                     Hkv)
@@ -140,8 +141,8 @@ def flash_attn_with_kvcache_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cac
                 nbytes, err, stream), "paged_decode_logits")
         check(lib().slokv_kv_scores_accumulate(
             scores.data_ptr(), row, head, width, rows, rows_ptr, logits, stride, int(four), lse,
-            cache_seqlens.data_ptr(), B, Hq, Hkv, block_table.shape[1] * bs, float(decay), err,
-            stream), "kv_scores_accumulate")
+            cache_seqlens.data_ptr(), B, Hq, Hkv, reach, float(decay), err, stream),
+            "kv_scores_accumulate")
     return out
 
 

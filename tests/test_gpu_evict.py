@@ -381,3 +381,34 @@ def test_evict_past_one_group_of_words_a_warp(pkg, kind):
     assert torch.equal(gs.cpu().view(torch.int32), want_s.view(torch.int32))
     for pool, w in zip((kp, vp), want):
         assert torch.equal(pool.view(torch.int16), w.view(torch.int16))
+
+
+@pytest.mark.parametrize("kind", ["dense", "int4"])
+def test_scored_scratch_is_bounded_by_the_tables(pkg, kind):
+    """The scratch goes by what the block tables reach, not by the score table's width (here
+    1 GiB of it); the scores are those of a narrow table."""
+    lens, H, G, bs = [200, 130, 1, 256], 1, 16, 64
+    nb = sum((n + bs - 1) // bs for n in lens)
+    kp, vp = (any_pool(pkg, kind, 15 + i, nb, bs, H, torch.bfloat16) for i in range(2))
+    tables = make_tables(17, lens, bs, nb).cuda()
+    q = torch.from_numpy(det_normal(18, (4, 1, H * G, 128))).float().bfloat16().cuda()
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    narrow = torch.zeros(4, H, 256, device="cuda")
+    want = pkg.flash_attn_with_kvcache_scored(q, kp, vp, narrow, ln, tables)
+    wide = torch.zeros(4, H, 2 ** 22, device="cuda")
+    pkg.read_device_errors()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = pkg.flash_attn_with_kvcache_scored(q, kp, vp, wide, ln, tables)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 2 ** 26      # the decode's workspace, mostly
+    assert torch.equal(out, want) and torch.equal(wide[:, :, :256], narrow)
+    assert not wide[:, :, 256:].any() and pkg.read_device_errors() == 0
+    # a context past the tables' reach is cut and flagged (and so is the padding of its table
+    # row, which it runs over), as on a narrow table
+    ln[2] = 300
+    pkg.flash_attn_with_kvcache_scored(q, kp, vp, wide, ln, tables, decay=0.0)
+    assert pkg.read_device_errors() == 0x6 and not wide[:, :, 256:].any()
+    pkg.flash_attn_with_kvcache_scored(q, kp, vp, narrow, ln, tables, decay=0.0)
+    assert pkg.read_device_errors() == 0x6 and torch.equal(wide[:, :, :256], narrow)
