@@ -42,7 +42,7 @@ extern "C" {
 #define SLOKV_DEVERR_BLOCK_RANGE  0x2u  /* block_tables entry outside [0, num_blocks) */
 #define SLOKV_DEVERR_CONTEXT_LEN  0x4u  /* context length > table width * block_size */
 #define SLOKV_DEVERR_TIMEOUT      0x8u  /* a bounded wait (mbarrier, peer flag) gave up */
-#define SLOKV_DEVERR_NONFINITE    0x10u /* FP8 encode met NaN/Inf (stored as code 0x7F) */
+#define SLOKV_DEVERR_NONFINITE    0x10u /* a quantising store met NaN/Inf, or a value past f16 was widened to it */
 
 /* ---- element types --------------------------------------------------------- */
 #define SLOKV_DTYPE_BF16      0
@@ -434,7 +434,9 @@ int slokv_int4_decode(const void *cache, int64_t block_stride, const int32_t *sl
  * dst_k / dst_v ([num_rows * pages_per_row, 128, num_kv_heads, 128], bf16 or f16),
  * token t of row r in page r * pages_per_row + t / 128, and dst_table ([num_rows,
  * pages_per_row]) is filled with those page ids, ready for slokv_paged_prefill
- * (block_size 128).  Values are rounded once to dst_dtype.  Pages that a row reaches
+ * (block_size 128).  Values are rounded once to dst_dtype; to f16, values up to 66,112,
+ * as far as rows stored from f16 can read, become at most 65,504, and larger ones
+ * infinite, with SLOKV_DEVERR_NONFINITE.  Pages that a row reaches
  * are written whole (zeros past its keys), the others not at all.  A block id
  * outside the pool reads as zeros and sets SLOKV_DEVERR_BLOCK_RANGE; so do keys past
  * the table's reach, with SLOKV_DEVERR_CONTEXT_LEN. */

@@ -234,7 +234,13 @@ __global__ void __launch_bounds__(kThreads)
 // beside them.  One CTA per (page, head, side).  A page that the row reaches is
 // written whole (zeros past its last key and for a block id outside the pool: the
 // prefill loads whole pages); the others are left alone.
+//
+// f16: a row of finite f16 can read back past 65,504: its minimum is rounded to bf16 (up by
+// 128 at most, down to -65,536) and so is its scale (half a step is 32 at most, 15 scales 480),
+// which makes 65,504 + 608 = 66,112 at most.  Those values are clamped, towards what was
+// stored; larger ones, of pools written in other types, become infinite and are flagged.
 constexpr int kWidePage = 128;
+constexpr float kF16Max = 65504.f, kF16Reach = 66112.f;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -277,6 +283,7 @@ __global__ void __launch_bounds__(kThreads)
     else if (i == 0)
       record_error(err, SLOKV_DEVERR_BLOCK_RANGE);
   }
+  bool past = false;                              // a value that f16 cannot hold
 #pragma unroll
   for (int k = 0; k < kSteps; ++k) {
     T *o = dst + static_cast<int64_t>(k * kWideRows + (threadIdx.x >> 3)) * hkv * kHeadDim + i * 8;
@@ -284,6 +291,13 @@ __global__ void __launch_bounds__(kThreads)
     for (int grp = 0; grp < 2; ++grp) {
       float v[8];
       piece_values(piece[k], grp, v);
+      if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {             // (NaN passes both tests unchanged)
+          past |= fabsf(v[e]) > kF16Reach;
+          if (fabsf(v[e]) <= kF16Reach) v[e] = fminf(fmaxf(v[e], -kF16Max), kF16Max);
+        }
+      }
       uint4 w;
       w.x = Mma<T>::pack(v[0], v[1]);
       w.y = Mma<T>::pack(v[2], v[3]);
@@ -292,6 +306,7 @@ __global__ void __launch_bounds__(kThreads)
       *reinterpret_cast<uint4 *>(o + 64 * grp) = w;
     }
   }
+  if (past) record_error(err, SLOKV_DEVERR_NONFINITE);
 }
 
 // The queries of a short prefill as decode rows: query token i of row r attends to the

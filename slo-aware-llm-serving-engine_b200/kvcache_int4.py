@@ -215,9 +215,10 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
     Arguments as flash_attn_varlen_func's paged form, any block_size that the pool
     allows.  Short calls (SHORT_CHUNK, SHORT_CALL) run as decode rows, one a query
     token.  For longer ones the rows' cached tokens are widened once to q's type (one
-    rounding) in a scratch of at most 1 GiB (or one row of max_seqlen_k tokens), as many
-    rows at a time as fit, which the tcgen05 prefill then reads: a few per cent of its
-    time when a chunk is a thousand tokens.
+    rounding; f16 queries on a pool with values past f16's range, which no f16 rows leave
+    in it, get infinities and the device error NONFINITE) in a scratch of at most 1 GiB (or
+    one row of max_seqlen_k tokens), as many rows at a time as fit, which the tcgen05
+    prefill then reads: a few per cent of its time when a chunk is a thousand tokens.
     """
     if block_table is None:
         raise SlokvError("4-bit varlen attention reads the pool: block_table is required")
