@@ -207,18 +207,28 @@ def flash_attn_with_kvcache_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache
     return out
 
 
+def _rows_on(x: torch.Tensor, align: int) -> bool:
+    """Whether every (token, head) row of x begins on a multiple of `align` bytes."""
+    es = x.element_size()
+    return not (x.data_ptr() | x.stride(0) * es | x.stride(1) * es) & (align - 1)
+
+
 def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
                                 max_seqlen_k, softmax_scale=None, causal=True, block_table=None,
                                 out=None):
     """Causal varlen attention over a 4-bit pool's pages (block_table required).
 
     Arguments as flash_attn_varlen_func's paged form, any block_size that the pool
-    allows.  Short calls (SHORT_CHUNK, SHORT_CALL) run as decode rows, one a query
-    token.  For longer ones the rows' cached tokens are widened once to q's type (one
-    rounding; f16 queries on a pool with values past f16's range, which no f16 rows leave
-    in it, get infinities and the device error NONFINITE) in a scratch of at most 1 GiB (or
-    one row of max_seqlen_k tokens), as many rows at a time as fit, which the tcgen05
-    prefill then reads: a few per cent of its time when a chunk is a thousand tokens.
+    allows.  q and out may be views at any address and stride with a contiguous last dim:
+    one that the call's kernel does not take (short calls: rows on 4 bytes, others: on 16)
+    goes through a contiguous copy.
+
+    Short calls (SHORT_CHUNK, SHORT_CALL) run as decode rows, one a query token.  For
+    longer ones the rows' cached tokens are widened once to q's type (one rounding; f16
+    queries on a pool with values past f16's range, which no f16 rows leave in it, get
+    infinities and the device error NONFINITE) in a scratch of at most 1 GiB (or one row
+    of max_seqlen_k tokens), as many rows at a time as fit, which the tcgen05 prefill then
+    reads: a few per cent of its time when a chunk is a thousand tokens.
     """
     if block_table is None:
         raise SlokvError("4-bit varlen attention reads the pool: block_table is required")
@@ -251,9 +261,18 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
         return out
     if block_table.shape[1] == 0:
         raise SlokvError("block_table has no columns")
-    if ((max_seqlen_q <= SHORT_CHUNK or Tq <= SHORT_CALL) and Tq <= _MAX_DECODE_ROWS
-            and Hq // Hkv <= _MAX_GROUP
-            and Tq * Hkv * block_table.shape[1] * (bs // TILE_TOKENS) < 2 ** 31):
+    short = ((max_seqlen_q <= SHORT_CHUNK or Tq <= SHORT_CALL) and Tq <= _MAX_DECODE_ROWS
+             and Hq // Hkv <= _MAX_GROUP
+             and Tq * Hkv * block_table.shape[1] * (bs // TILE_TOKENS) < 2 ** 31)
+    if not _rows_on(q, 4 if short else 16):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if not _rows_on(out, 4 if short else 16):
+        # (a copy with out's content, since tokens of no row keep it)
+        res = out.clone(memory_format=torch.contiguous_format)
+        flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
+                                    max_seqlen_k, softmax_scale, causal, block_table, res)
+        return out.copy_(res)
+    if short:
         scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
         with on_device(dev) as stream:
             nbytes = decode_int4_workspace_bytes(dev.index, Hq, Hkv)

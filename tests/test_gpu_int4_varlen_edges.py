@@ -29,6 +29,51 @@ def check_long(out, q, k, v, seen, dtype):
         assert (err <= (2 * half + 2.0 ** -13) * wv + 2.0 ** -25).all(), (i, (err - 2 * half * wv).max())
 
 
+def place(raw, at, shape, strides):
+    """A view of the flat tensor `raw` that starts at element `at`."""
+    return torch.as_strided(raw, shape, strides, raw.storage_offset() + at)
+
+
+@pytest.mark.parametrize("T", [61, 64, 65])           # 64 query tokens in all; 67; 68
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at,row,head", [
+    (0, 1024, 128),                  # contiguous
+    (4, 1024, 128),                  # 8 bytes off
+    (1, 1024, 128),                  # an odd element
+    (0, 1540, 128),                  # rows of a fused projection, 8 bytes off a multiple of 16
+    (8, 1600, 130),                  # heads 4 bytes off
+    (2, 1601, 131),                  # neither rows nor heads on 4 bytes
+    (0, 1024, 0),                    # one head's query for all (q only)
+])
+def test_varlen_any_view(pkg, T, dtype, at, row, head):
+    """q and out at any address and stride give what contiguous ones do; rows behind the last
+    sequence and the elements between out's rows keep what they held."""
+    H, G, bs, klen, more = 2, 4, 64, 150, 3
+    kp, vp = make_pool(pkg, 1, 4, bs, H), make_pool(pkg, 2, 4, bs, H)
+    tables = make_tables(3, [klen], bs, 4).cuda()
+    n = T + more
+    raw = torch.from_numpy(det_normal(4, (at + n * max(row, 1024) + 2048,))).float().to(dtype).cuda()
+    q = place(raw, at, (n, H * G, 128), (row, head, 1))
+    if head:
+        held = torch.full_like(raw, 7.0)
+        out = place(held, at, (n, H * G, 128), (row, head, 1))
+    else:
+        held, out = None, torch.full((n, H * G, 128), 7.0, dtype=dtype, device="cuda")
+    args = (kp, vp, i32(0, T), i32(0, klen), T, klen)
+    pkg.read_device_errors()
+    want = torch.full((n, H * G, 128), 7.0, dtype=dtype, device="cuda")
+    pkg.flash_attn_varlen_func_int4(q.clone(memory_format=torch.contiguous_format), *args,
+                                    block_table=tables, out=want)
+    res = pkg.flash_attn_varlen_func_int4(q, *args, block_table=tables, out=out)
+    assert res.data_ptr() == out.data_ptr() and pkg.read_device_errors() == 0
+    assert torch.equal(out, want) and (out[T:] == 7).all()
+    if held is not None:
+        out.fill_(7.0)
+        assert (held == 7).all()
+    fresh = pkg.flash_attn_varlen_func_int4(q, *args, block_table=tables)
+    assert torch.equal(fresh[:T], want[:T])
+
+
 @pytest.mark.parametrize("T", [64, 70])
 def test_varlen_values_at_the_end_of_f16(pkg, T):
     """f16 rows whose values read back past f16's largest (the minimum -65,504 is stored as
