@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/slokv.h"
 
 namespace slokv {
@@ -194,6 +196,19 @@ __device__ __forceinline__ void launch_dependents() {
 }
 __device__ __forceinline__ void wait_prerequisites() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// The attributes of a function (its limit of dynamic shared memory) hold on one device: `set`
+// runs on the first call on each, and again after a failure.  `done`: the devices that have it.
+template <typename F>
+inline bool once_per_device(std::atomic<uint64_t> &done, F set) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (!set()) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 // Launch `kernel`, which starts with wait_prerequisites, without waiting for the end of the

@@ -30,7 +30,6 @@
 
 #include <cudaTypedefs.h>
 
-#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -787,19 +786,14 @@ int launch(const Params &p0, const CUtensorMap &km, const CUtensorMap &vm, int s
   constexpr int kW = Ring<kFp8>::kWarpsPerCta;
   const size_t smem = 1024 + kRingBytes + kW * Ring<kFp8>::kStages * 8 +
                       static_cast<size_t>(p0.batch + 1) * sizeof(int32_t);
-  // The limit is an attribute of the function on one device: set on the first call there.
-  static std::atomic<uint64_t> set{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return SLOKV_ERR_CUDA;
-  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-  if (!(set.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(paged_decode_kernel<T, kFp8, kScored>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             1024 + kRingBytes + kW * Ring<kFp8>::kStages * 8 +
-                                 (kMaxBatch + 1) * sizeof(int32_t)) != cudaSuccess)
-      return SLOKV_ERR_CUDA;
-    set.fetch_or(bit, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> done{0};
+  const bool ok = once_per_device(done, [] {
+    return cudaFuncSetAttribute(paged_decode_kernel<T, kFp8, kScored>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                1024 + kRingBytes + kW * Ring<kFp8>::kStages * 8 +
+                                    (kMaxBatch + 1) * sizeof(int32_t)) == cudaSuccess;
+  });
+  if (!ok) return SLOKV_ERR_CUDA;
   paged_decode_kernel<T, kFp8, kScored><<<sms, kW * 32, smem, stream>>>(km, vm, p0);
   if (cudaGetLastError() != cudaSuccess) return SLOKV_ERR_CUDA;
   if (kScored)

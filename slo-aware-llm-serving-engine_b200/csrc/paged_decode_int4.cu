@@ -51,7 +51,6 @@
 #include "decode_worklist.cuh"
 #include "int4_page.cuh"
 
-#include <atomic>
 #include <type_traits>
 
 namespace slokv {
@@ -945,18 +944,15 @@ size_t smem_bytes(int warps, int batch) {
 }
 
 template <typename T, int kN, bool kScored>
-int launch(const Params &p, int dev, int sms, cudaStream_t stream) {
+int launch(const Params &p, int sms, cudaStream_t stream) {
   constexpr int kWarps = warps_of(kN);
-  // The limit is an attribute of the function on one device: set on the first call there.
-  static std::atomic<uint64_t> set{0};
-  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-  if (!(set.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(paged_decode_int4_kernel<T, kN, kScored>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem_bytes(kWarps, kMaxBatch))) != cudaSuccess)
-      return SLOKV_ERR_CUDA;
-    set.fetch_or(bit, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> done{0};
+  const bool ok = once_per_device(done, [] {
+    return cudaFuncSetAttribute(paged_decode_int4_kernel<T, kN, kScored>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(smem_bytes(kWarps, kMaxBatch))) == cudaSuccess;
+  });
+  if (!ok) return SLOKV_ERR_CUDA;
   paged_decode_int4_kernel<T, kN, kScored><<<sms, kWarps * 32, smem_bytes(kWarps, p.batch),
                                             stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SLOKV_ERR_CUDA;
@@ -968,10 +964,10 @@ int launch(const Params &p, int dev, int sms, cudaStream_t stream) {
 }
 
 template <typename T>
-int pick(const Params &p, bool scored, int dev, int sms, cudaStream_t st) {
+int pick(const Params &p, bool scored, int sms, cudaStream_t st) {
   if (p.group <= 8)
-    return scored ? launch<T, 1, true>(p, dev, sms, st) : launch<T, 1, false>(p, dev, sms, st);
-  return scored ? launch<T, 2, true>(p, dev, sms, st) : launch<T, 2, false>(p, dev, sms, st);
+    return scored ? launch<T, 1, true>(p, sms, st) : launch<T, 1, false>(p, sms, st);
+  return scored ? launch<T, 2, true>(p, sms, st) : launch<T, 2, false>(p, sms, st);
 }
 
 }  // namespace decode4
@@ -1066,6 +1062,6 @@ extern "C" int slokv_paged_decode_int4(void *out, int64_t out_stride_b, int64_t 
   p.err = dev_error;
   p.nslots = sms * warps_for(group);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return q_dtype == SLOKV_DTYPE_BF16 ? pick<__nv_bfloat16>(p, logits != nullptr, dev, sms, st)
-                                     : pick<__half>(p, logits != nullptr, dev, sms, st);
+  return q_dtype == SLOKV_DTYPE_BF16 ? pick<__nv_bfloat16>(p, logits != nullptr, sms, st)
+                                     : pick<__half>(p, logits != nullptr, sms, st);
 }

@@ -1402,19 +1402,23 @@ bool encode_code_map(CUtensorMap *map, const void *base, uint64_t heads, uint64_
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Registers a thread of `kernel` as built; -1 if the query fails.
+template <typename K>
+int launch_registers(K kernel) {
+  cudaFuncAttributes fa;
+  return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : -1;
+}
+
 template <typename Tq>
 int launch_fp8(const Params &p, const CUtensorMap &qm, const CUtensorMap &km,
                const CUtensorMap &vm, int rows, cudaStream_t stream) {
-  static std::once_flag once;
-  static bool ok = false;
-  std::call_once(once, [] {
-    cudaFuncAttributes fa;
+  static std::atomic<uint64_t> done{0};
+  const bool ok = once_per_device(done, [] {
     // the register split hands out exactly the launch allocation (see f8::kRegsLaunch)
-    ok = cudaFuncSetAttribute(paged_prefill_fp8_kernel<Tq>,
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, ws::kSmemMax) ==
-             cudaSuccess &&
-         cudaFuncGetAttributes(&fa, paged_prefill_fp8_kernel<Tq>) == cudaSuccess &&
-         fa.numRegs == f8::kRegsLaunch;
+    return cudaFuncSetAttribute(paged_prefill_fp8_kernel<Tq>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, ws::kSmemMax) ==
+               cudaSuccess &&
+           launch_registers(paged_prefill_fp8_kernel<Tq>) == f8::kRegsLaunch;
   });
   if (!ok) return SLOKV_ERR_UNSUPPORTED;
   const int64_t smem = f8::kSmemFixed + 8 * static_cast<int64_t>(p.max_blocks);
@@ -1432,27 +1436,23 @@ int launch_fp8(const Params &p, const CUtensorMap &qm, const CUtensorMap &km,
 template <typename T>
 int launch(const Params &p, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm,
            int rows, int max_q, cudaStream_t stream) {
-  static std::once_flag once;
-  static bool ok = false, ws_ok = false, ws_scaled_ok = false;
-  std::call_once(once, [] {
-    ok = cudaFuncSetAttribute(paged_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              kSmemBytes) == cudaSuccess &&
-         cudaFuncSetAttribute(paged_prefill_ws_kernel<T, false>,
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, ws::kSmem) == cudaSuccess &&
-         cudaFuncSetAttribute(paged_prefill_ws_kernel<T, true>,
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, ws::kSmemMax) ==
-             cudaSuccess;
-    // The register split in the two-head kernel hands out exactly the launch
-    // allocation; with any other per-thread count setmaxnreg.inc could not be
-    // satisfied, so that kernel is used only when the build matches.
-    cudaFuncAttributes fa;
-    ws_ok = ok && cudaFuncGetAttributes(&fa, paged_prefill_ws_kernel<T, false>) == cudaSuccess &&
-            fa.numRegs == ws::kRegsLaunch;
-    ws_scaled_ok = ok &&
-                   cudaFuncGetAttributes(&fa, paged_prefill_ws_kernel<T, true>) == cudaSuccess &&
-                   fa.numRegs == ws::kRegsLaunch;
+  static std::atomic<uint64_t> done{0};
+  const bool ok = once_per_device(done, [] {
+    return cudaFuncSetAttribute(paged_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kSmemBytes) == cudaSuccess &&
+           cudaFuncSetAttribute(paged_prefill_ws_kernel<T, false>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, ws::kSmem) == cudaSuccess &&
+           cudaFuncSetAttribute(paged_prefill_ws_kernel<T, true>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, ws::kSmemMax) ==
+               cudaSuccess;
   });
   if (!ok) return SLOKV_ERR_CUDA;
+  // The register split in the two-head kernel hands out exactly the launch
+  // allocation; with any other per-thread count setmaxnreg.inc could not be
+  // satisfied, so that kernel is used only when the build matches.
+  static const bool ws_ok = launch_registers(paged_prefill_ws_kernel<T, false>) == ws::kRegsLaunch;
+  static const bool ws_scaled_ok =
+      launch_registers(paged_prefill_ws_kernel<T, true>) == ws::kRegsLaunch;
   const bool scaled = p.k_page_scale != nullptr;
   if (scaled && !(p.group % 2 == 0 && ws_scaled_ok)) return SLOKV_ERR_UNSUPPORTED;
   const int64_t smem_scaled = ws::kSmem + 4 * static_cast<int64_t>(p.max_blocks);
