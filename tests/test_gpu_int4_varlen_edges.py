@@ -74,6 +74,32 @@ def test_varlen_any_view(pkg, T, dtype, at, row, head):
     assert torch.equal(fresh[:T], want[:T])
 
 
+@pytest.mark.parametrize("nq", [3, 66])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_varlen_rows_around_and_values(pkg, nq, dtype):
+    """Query tokens before the first and behind the last row keep what `out` held, those without
+    keys give zeros, the others their attention."""
+    H, G, bs, first = 1, 2, 64, 3
+    kp, vp = make_pool(pkg, 5, 4, bs, H), make_pool(pkg, 6, 4, bs, H)
+    n = first + nq + 4
+    q = torch.from_numpy(det_normal(7, (n, H * G, 128))).float().to(dtype)
+    out = torch.full((n, H * G, 128), 5.0, dtype=dtype, device="cuda")
+    pkg.read_device_errors()
+    pkg.flash_attn_varlen_func_int4(q.cuda(), kp, vp, i32(first, first + nq), i32(0, nq - 2), nq, nq - 2,
+                                    block_table=i32(3).view(1, 1), out=out)
+    assert pkg.read_device_errors() == 0
+    out = out.cpu()
+    last = first + nq
+    assert (out[:first] == 5).all() and (out[last:] == 5).all() and (out[first:first + 2] == 0).all()
+    seen = list(range(1, nq - 1))
+    mine, mq = out[first + 2:last], q[first + 2:last]
+    if nq <= 64:
+        check_decode(mine.unsqueeze(1), mq.unsqueeze(1), kp, vp, seen, torch.full((nq, 1), 3), SCALE)
+    else:
+        k, v = (R.gather(R.decode_pool(p.cpu())[0], [3], nq - 2).to(dtype).double() for p in (kp, vp))
+        check_long(mine, mq, k, v, seen, dtype)
+
+
 @pytest.mark.parametrize("T", [64, 70])
 def test_varlen_values_at_the_end_of_f16(pkg, T):
     """f16 rows whose values read back past f16's largest (the minimum -65,504 is stored as
