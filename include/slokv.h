@@ -407,6 +407,9 @@ int slokv_kv_block_copy(const void *src, int64_t src_plane_stride_bytes,
  * Quantising append (every step in fp32, round to nearest even):
  *   scale = bf16((max - min) / 15), minimum = bf16(min),
  *   code = scale > 0 ? clamp(rint((x - minimum) / scale), 0, 15) : 0.
+ * A stored value is half a scale from x at most, for bf16 rows and where |min| is up to
+ * 7 (max - min); f16 and fp32 rows further from zero than that lose up to 2^-8 (|min| +
+ * max - min), since their minimum is rounded to bf16 and the outermost codes clamp.
  * A group with a NaN or infinity, or whose range overflows fp32, gets a NaN scale
  * (its values read as NaN) and sets SLOKV_DEVERR_NONFINITE.  Nothing but the stored
  * tokens' own bytes is written, so a reused page needs no reset.  Slot -1 skips; the

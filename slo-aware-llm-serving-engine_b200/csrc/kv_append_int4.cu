@@ -5,6 +5,8 @@
 //   mn = min x, mx = max x
 //   scale = bf16((mx - mn) / 15), minimum = bf16(mn)
 //   code = scale > 0 ? clamp(rint((x - minimum) / scale), 0, 15) : 0
+// The value is within half a scale of x, except that f16 and fp32 groups with |min| > 7 (mx -
+// mn) clamp where bf16(min) misses min: within 2^-8 (|min| + mx - mn).
 // A group with a NaN or an infinity, or whose range overflows fp32, is stored with a
 // NaN scale (its values read as NaN) and flags SLOKV_DEVERR_NONFINITE.  A token's
 // parameters are its own, so nothing stored before is touched and a page needs no

@@ -82,6 +82,10 @@ def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
     key / value: [N, Hkv, 128] bf16, f16 or fp32 (the same type), any row and head
     strides with a contiguous last dim (views of a fused qkv projection too);
     slot_mapping: [N] int32, -1 skips the token, the other slots distinct.
+
+    A value comes back within half a step (a fifteenth of its group's range, rounded), but
+    f16 and fp32 groups whose |min| is more than 7 times their range come back within
+    2^-8 (|min| + range): their minimum is kept in bf16.
     """
     if key.dim() != 3 or value.shape != key.shape:
         raise SlokvError("key and value must be [tokens, heads, head_dim] of one shape")
@@ -228,7 +232,9 @@ def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
     queries on a pool with values past f16's range, which no f16 rows leave in it, get
     infinities and the device error NONFINITE) in a scratch of at most 1 GiB (or one row
     of max_seqlen_k tokens), as many rows at a time as fit, which the tcgen05 prefill then
-    reads: a few per cent of its time when a chunk is a thousand tokens.
+    reads: a few per cent of its time when a chunk is a thousand tokens.  There, as in
+    flash_attn_varlen_func, a V row that is not finite (the store flags it) also reaches
+    the queries of its 128-key tile that come before it.
     """
     if block_table is None:
         raise SlokvError("4-bit varlen attention reads the pool: block_table is required")

@@ -207,6 +207,34 @@ def test_store_slot_out_of_range(pkg):
     assert (got[:3] == 0).all() and (got[3] == 1).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("amp,bias", [(0.5, 0), (0.5, 4), (0.5, 16), (0.5, 64), (0.5, -64), (3.0, 1000),
+                                      (1e-3, -1000), (200.0, 100)])
+def test_store_offset_rows(pkg, dtype, amp, bias):
+    """How far a stored value lies from its input, with R the group's range and s its scale.  A code
+    that is not clamped is half a step s off.  The minimum may be 2^-8 |min| off (bf16 rows: not
+    at all) and 15 s below R by 2^-8 R, so a clamped one is 2^-8 (|min| + R) off at most, which is
+    less than half a step while |min| <= 7 R: s / 2 >= R / 30 (1 - 2^-8) > 0.033 R and 2^-8 8 R
+    < 0.0313 R.  The quotient is 2^-20 of a step off its border, the fp32 value 2^-24 of itself."""
+    T, H, bs = 24, 2, 64
+    x = (torch.from_numpy(det_normal(int(abs(bias)) + 3, (T, H, 128))).float() * amp + bias).to(dtype)
+    kp = torch.zeros(pkg.int4_pool_shape(1, bs, H), dtype=torch.uint8, device="cuda")
+    vp = torch.zeros_like(kp)
+    slots = torch.arange(T, dtype=torch.int32, device="cuda")
+    pkg.store_kvcache_int4(x.cuda(), x.cuda(), kp, vp, slots)
+    got = pkg.int4_decode(kp, slots).cpu().double().view(T, H, 2, 64)
+    scale = R.decode_pool(kp.cpu())[1][0, :T].unsqueeze(-1)               # [T, H, 2, 1]
+    v = x.double().view(T, H, 2, 64)
+    low = v.amin(-1, keepdim=True)
+    span, low = v.amax(-1, keepdim=True) - low, low.abs()
+    clamped = 2.0 ** -8 * ((low if dtype != torch.bfloat16 else 0) + span)
+    half = 0.5 * scale * (1 + 2.0 ** -19)
+    bound = torch.where(low <= 7 * span, half, torch.maximum(half, clamped))
+    if dtype == torch.bfloat16:
+        bound = half.expand_as(span)
+    assert ((got - v).abs() <= bound + 2.0 ** -23 * v.abs()).all()
+
+
 # ---- decode ----------------------------------------------------------------------
 
 LENS = [[1], [64, 65, 63, 0, 1, 128], [0, 0], [700, 5, 1023, 0, 129], [4500]]
