@@ -212,9 +212,9 @@ def flash_attn_with_kvcache_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache
 
 
 def _rows_on(x: torch.Tensor, align: int) -> bool:
-    """Whether every (token, head) row of x begins on a multiple of `align` bytes."""
-    es = x.element_size()
-    return not (x.data_ptr() | x.stride(0) * es | x.stride(1) * es) & (align - 1)
+    """Whether every (token, head) row of x, bf16 or f16, begins on a multiple of `align` bytes."""
+    row, head, _ = x.stride()
+    return not (x.data_ptr() | row * 2 | head * 2) & (align - 1)
 
 
 def flash_attn_varlen_func_int4(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
