@@ -531,8 +531,8 @@ int slokv_kv_scores_accumulate(float *scores, int64_t row_stride, int64_t head_s
  *
  * cache_dtype: SLOKV_DTYPE_BF16, _F16, _F32 ([num_blocks, block_size, num_kv_heads, 128])
  * or _INT4; block strides in bytes; pools 16-byte aligned.  1 <= keep, 0 <= recent
- * <= keep.  The blocks below position keep must belong to one sequence only (copy
- * shared ones first).  A sequence whose score row is -1 or outside [0, num_score_rows)
+ * <= keep.  The blocks below position keep and the score rows must belong to one
+ * sequence only (copy shared blocks first).  A sequence whose score row is -1 or outside [0, num_score_rows)
  * or whose context exceeds the table's or the score row's width is left as it is
  * (new_lens[b] = L_b), the latter two with SLOKV_DEVERR_SLOT_RANGE / _CONTEXT_LEN; a
  * move whose block id lies outside the pool is dropped with

@@ -75,7 +75,8 @@ constexpr int kFlush = 8;                                 // tiles between two m
 constexpr int kSkip = 4;                                  // sequences per entry of the tile prefix
 
 // Warps of a CTA by the query-head columns (kN x 8): twice the accumulators at kN = 2 need
-// the larger register share of 8 warps.
+// the larger register share of 8 warps, and spill a little even so (128 sequences of 1,024-8,192
+// tokens, 721 MB, 16 heads a KV head: 212 us in bf16, 260 in f16; 8 heads: 137 in bf16).
 constexpr int warps_of(int kN) { return kN == 1 ? 12 : 8; }
 constexpr int ring_bytes(int warps) { return warps * kStages * kStage; }
 

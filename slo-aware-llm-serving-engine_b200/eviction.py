@@ -158,8 +158,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     zeroed.  Returns the new lengths ([B] int32) and, with return_index, the position
     that each slot's token came from ([B, Hkv, keep] int32, -1 past the new length).
 
-    The pages below position keep must belong to one sequence each (kv_block_copy
-    shared ones first); those past it can be freed afterwards.
+    The pages below position keep and the score rows must belong to one sequence each
+    (kv_block_copy shared pages first); the pages past it can be freed afterwards.
     """
     keep, recent = int(keep), int(recent)
     if not 1 <= keep < 2 ** 31 or not 0 <= recent <= keep:

@@ -11,11 +11,12 @@ kv_cache[0, l] / kv_cache[1, l].
 
 FP8-E4M3 pools keep uint8 codes in the same layout plus fp32 scales
 k_scale/v_scale [num_layers, num_blocks, Hkv_local]; block_bytes counts the
-scales.  4-bit pools are one uint8 tensor [2, num_layers, num_blocks, Hkv_local,
-block_size * 72] whose pages carry their own scales.  A reused page never inherits an old amax without any call from the
+scales.  A reused page never inherits an old amax without any call from the
 block manager: the quantising append ignores a block's stored scale when its
 write starts at offset 0, where every newly assigned block is first written
 (reset_blocks remains as an eager helper for tools that want clean scales).
+4-bit pools are one uint8 tensor [2, num_layers, num_blocks, Hkv_local,
+block_size * 72] whose pages carry their own scales.
 """
 from __future__ import annotations
 
