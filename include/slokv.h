@@ -452,7 +452,8 @@ int slokv_int4_rows_widen(const void *k_cache, const void *v_cache, int64_t k_bl
                           uint32_t *dev_error, void *stream);
 
 /* Paged decode over a 4-bit pool: slokv_paged_decode's arguments and result with
- * the pool as above.  q / out are bf16 or f16 (q_dtype), at most 16 query heads per
+ * the pool as above.  q / out are bf16 or f16 (q_dtype), |q| below 2^118 (q rows are
+ * brought to f16's range by a power of two that fp32 scores undo), at most 16 query heads per
  * KV head, batch at most 8192, batch * num_kv_heads * the table's reach in tiles of 64
  * tokens below 2^31 (else SLOKV_ERR_UNSUPPORTED).  table_rows: NULL, or the block
  * table row of each sequence; with it a context length of -1 leaves the sequence's
